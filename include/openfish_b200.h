@@ -179,6 +179,118 @@ int openfish_b200_decode_static(int T, int N, int C, const void *scores_TNC, int
                                 const openfish_opt_t *options, uint8_t *moves_gpu,
                                 char *sequence_gpu, char *qstring_gpu);
 
+/* ---- Operators of the transformer encoder in front of the CRF head.  Next to openfish_rotary_emb_gpu they
+ * make up a layer of it: the tokens are brought to 8 bits (norm, kind NONE), projected to Q, K and V
+ * (matmul_i8), Q and K rotated, attention taken within every chunk or read (attention), the result projected
+ * back, and the sum with the residual normalised (norm).  No counterpart in the reference, which has only the
+ * rotary embedding.
+ *
+ * What they share:
+ *   - cuda_stream is the caller's stream (a cudaStream_t; NULL is the legacy default stream) on the calling
+ *     thread's current device, on which every pointer of the call lives.  The call queues its kernels there and returns; it
+ *     allocates nothing, waits for nothing, keeps nothing of its arguments and may be captured into a graph
+ *     (the graph then holds the pointers).  The struct itself may go once the call has returned.
+ *   - Buffers must not overlap, except where a field says so; a workspace belongs to one call until that call's kernels are
+ *     done, so calls that may run at the same time (two streams, two graphs) need one each.  Its contents need no
+ *     preparation.
+ *   - Strides are in elements.  Arguments that cannot be served are refused before anything is queued
+ *     (openfish_b200_last_status, the library's error mode).
+ *   - Sums, statistics and scales are held in 32 bits; a result is rounded to its type once. */
+enum openfish_b200_dtype { OPENFISH_B200_F16 = 0, OPENFISH_B200_BF16 = 1 };
+
+/* Attention over packed sequences.
+ *
+ *   out[i][h] = sum_j p_ij v[j][h / g],   p_ij = softmax over j of scale * <q[i][h], k[j][h / g]>,   g = q_heads / kv_heads,
+ *
+ * for query i of a sequence over those keys j of the same sequence with
+ * place(i) - window_left <= j <= place(i) + window_right, where place(i) = i + (number of keys) - (number of
+ * queries): the sequences' ends fall together.  A window of -1 has no bound; window_right = 0 is causal attention,
+ * both -1 attention over the whole sequence, and one query against many keys is the step of a decoder with a
+ * cache.  <q, k> is a sum in fp32 before it is scaled; one beyond fp32 is an infinity, with what follows from that (a query all of whose keys give
+ * -inf has no softmax: NaN).  A query that sees no key gets zeros.  Keys that a query does not see have no part in its result, whatever
+ * their values (infinities and NaN included).
+ *
+ * q [q_rows][q_heads][head_dim], k and v [k_rows][kv_heads][head_dim], out like q, all of type `dtype`, the head_dim
+ * elements of a head next to each other, 16-byte aligned, strides multiples of 8 and positive.  head_dim: a multiple
+ * of 8 up to 128.  Sequence s has the queries q_start[s] .. q_start[s] + n - 1, n = q_used[s], or
+ * q_start[s + 1] - q_start[s] where q_used is NULL, and its keys likewise: q_used and k_used are for padded batches and
+ * caches with room left; they are cut to the room that the starts give.  Starts and used lengths are in device memory and are read by the kernels; starts have sequences + 1
+ * entries, do not fall, and lie in 0 .. rows.  Rows of out behind a sequence's last query are left as they were.
+ * max_q and max_k: at least the longest sequence's queries and keys (rows beyond them are not computed or not seen). */
+typedef struct openfish_b200_attention {
+    int dtype; /* openfish_b200_dtype */
+    int head_dim, q_heads, kv_heads;
+    int sequences, max_q, max_k;
+    int window_left, window_right;
+    float scale; /* above zero */
+    long long q_rows, k_rows;
+    const int32_t *q_start, *k_start;
+    const int32_t *q_used, *k_used; /* or NULL */
+    const void *q, *k, *v;
+    void *out;
+    long long q_stride_row, q_stride_head, k_stride_row, k_stride_head;
+    long long v_stride_row, v_stride_head, out_stride_row, out_stride_head;
+    void *workspace; /* 16-byte aligned; NULL where openfish_b200_attention_workspace says 0 */
+    size_t workspace_bytes;
+} openfish_b200_attention_t;
+/* Bytes of workspace that openfish_b200_attention takes for these sizes on the current device (the pointers are not looked
+ * at); 0 if it needs none or the arguments are refused. */
+size_t openfish_b200_attention_workspace(const openfish_b200_attention_t *args);
+void openfish_b200_attention(void *cuda_stream, const openfish_b200_attention_t *args);
+
+/* Product of tokens and weights in 8-bit integers:
+ *
+ *   out[m][n] = x_scale[m] * w_scale[n] * sum_k x[m][k] * w[n][k]  (+ bias[n])
+ *
+ * The sum is exact.  x [rows][depth], w [cols][depth] int8, each row on a 16-byte boundary (strides multiples of 16; what
+ * lies between depth and the stride is not used); depth up to 131071 (beyond, the sum could leave 32 bits).  x_scale [rows],
+ * w_scale [cols] fp32; bias [cols] or NULL and out [rows][cols] of type `dtype`. */
+typedef struct openfish_b200_matmul_i8 {
+    int dtype; /* of out and bias */
+    int cols, depth;
+    long long rows;
+    const int8_t *x, *w;
+    const float *x_scale, *w_scale;
+    const void *bias; /* or NULL */
+    void *out;
+    long long x_stride, w_stride, out_stride;
+    void *workspace; /* 16-byte aligned; NULL where openfish_b200_matmul_i8_workspace says 0 */
+    size_t workspace_bytes;
+} openfish_b200_matmul_i8_t;
+size_t openfish_b200_matmul_i8_workspace(const openfish_b200_matmul_i8_t *args);
+void openfish_b200_matmul_i8(void *cuda_stream, const openfish_b200_matmul_i8_t *args);
+
+/* Residual, norm and 8-bit tokens, row by row:
+ *
+ *   s = x + residual_scale * residual            (s = x where residual is NULL)
+ *   y = s                                        kind NONE
+ *   y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias      kind LAYER
+ *   y = s / sqrt(mean(s^2) + eps) * weight + bias               kind RMS
+ *
+ * weight and bias [width] or NULL (1 and 0; kind NONE takes neither).  out (or NULL): y in the type of x.  q (or NULL): y in
+ * 8 bits, q = round(y * 127 / top) to nearest, ties to even, and q_scale[row] = top / 127 with top = max |y| of the row (from the unrounded y); a row of zeros gets
+ * zeros and scale 0, a row with an infinity or NaN zeros and scale NaN.  width up to 32768.  out may be x or
+ * residual themselves (same pointer, same stride). */
+enum openfish_b200_norm_kind { OPENFISH_B200_NORM_NONE = 0, OPENFISH_B200_NORM_LAYER = 1, OPENFISH_B200_NORM_RMS = 2 };
+typedef struct openfish_b200_norm {
+    int dtype; /* of x, residual, weight, bias and out */
+    int kind;  /* openfish_b200_norm_kind */
+    int width;
+    float eps, residual_scale;
+    long long rows;
+    const void *x, *residual, *weight, *bias;
+    void *out;
+    int8_t *q;
+    float *q_scale;
+    long long x_stride, residual_stride, out_stride, q_stride;
+} openfish_b200_norm_t;
+void openfish_b200_norm(void *cuda_stream, const openfish_b200_norm_t *args);
+
+/* Waits for cuda_stream and reports whether a kernel of the three operators has given up waiting for a copy or a matrix
+ * instruction on this device since the last such call (OPENFISH_B200_ERR_DEVICE_WAIT; results queued since are then
+ * meaningless).  The operators themselves do not wait and cannot tell.  Not while a capture is under way. */
+void openfish_b200_encoder_wait(void *cuda_stream);
+
 /* The four helpers the reference's test driver (src/main.c:207-252,337-351) calls next to the
  * public API; the reference declares them in an internal header (src/decode_cuda.h:35-55).
  * Same names, arguments and behaviour, so that a driver written against the reference links

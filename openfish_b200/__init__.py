@@ -12,6 +12,8 @@ import weakref
 
 import numpy as np
 
+from . import encoder as _encoder
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("OPENFISH_B200_LIB") or os.path.join(_HERE, "lib", "libopenfish.so")
 
@@ -102,6 +104,7 @@ def lib():
         L.openfish_b200_selfcheck_arith.argtypes = [C.POINTER(C.c_double)]
         L.openfish_b200_decode_static.restype = i
         L.openfish_b200_decode_static.argtypes = [i, i, i, vp, i, C.POINTER(Opt), vp, vp, vp]
+        _encoder.declare(L)
         L.get_openfish_log_level.restype = i
         L.set_openfish_log_level.argtypes = [i]
         # Python callers get exceptions instead of the reference's exit(1)
@@ -305,4 +308,5 @@ def last_rotary_ms():
     return float(lib().openfish_b200_last_rotary_ms())
 
 
+from .encoder import attention, encoder_wait, matmul_i8, norm, quantize_i8  # noqa: E402,F401
 from .sharding import shard_range  # noqa: E402,F401

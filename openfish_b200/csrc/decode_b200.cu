@@ -164,6 +164,7 @@ cudaError_t of_prepare_device() {
 }
 
 extern "C" const char *ofb_error_text(void) { return g_err; }
+extern "C" int ofb_fail(int code, const char *text) { return fail(code, "%s", text); }
 
 extern "C" int ofb_gpubuf_create(int T, int N, int state_len, openfish_gpubuf_t **out) {
     *out = nullptr;

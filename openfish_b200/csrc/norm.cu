@@ -1,0 +1,219 @@
+// norm.cu -- residual, norm and 8-bit tokens, row by row (openfish_b200_norm).
+//
+//   s = x + alpha r;  y = (s - mean) / sqrt(var + eps) w + b  (or without the mean, or y = s);  out = y in 16 bits;
+//   q = round(127 y / max|y|), scale = max|y| / 127
+//
+// One pass over memory: a row's s stays in the registers of the warp or block that read it, so the mean, the
+// variance about that mean (two sums, no cancellation), the largest |y| and the results all come from there.  What
+// bounds it is HBM: 2 bytes for each of x, r, out and 1 for q.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "encoder.h"
+#include "encoder_device.cuh"
+
+namespace {
+
+using ofe::from_float;
+using ofe::to_float;
+
+template <class T>
+struct NormArgs {
+    const T *x, *r, *w, *b;
+    T *out;
+    int8_t *q;
+    float *q_scale;
+    long long x_stride, r_stride, out_stride, q_stride, rows;
+    int width, kind;
+    float eps, alpha;
+};
+
+// V elements that lie together: 16 bytes where everything is aligned to that, else one at a time.
+template <class T, int V>
+struct alignas(V == 8 ? 16 : sizeof(T)) Pack {
+    T v[V];
+};
+template <int V>
+struct alignas(V) Pack8 {
+    int8_t v[V];
+};
+
+// A sum (or maximum) over the threads of a row: its warp, or all warps of the block through shared memory.
+template <bool BLOCK, class Op>
+__device__ __forceinline__ float reduce(float v, float *scratch, Op op) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, d));
+    if (BLOCK) {
+        const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+        __syncthreads();  // the last reduction's readers are done
+        if (lane == 0) scratch[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = scratch[lane < warps ? lane : 0];
+        // every warp adds the same numbers in the same order; lanes beyond the last warp hold the neutral element
+        if (lane >= warps) v = op(0.f, 0.f);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, d));
+    }
+    return v;
+}
+
+// BLOCK: a block to a row, else a warp.  CH packs of V elements to a thread.
+template <class T, int V, int CH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs<T> a) {
+    __shared__ float scratch[32];
+    const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
+    const int lanes = BLOCK ? blockDim.x : 32;
+    const long long step = BLOCK ? gridDim.x : (long long)gridDim.x * (blockDim.x >> 5);
+    const long long first = BLOCK ? blockIdx.x : (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const auto add = [](float p, float q) { return p + q; };
+    const auto most = [](float p, float q) { return fmaxf(p, q); };
+    const float inv = 1.f / (float)a.width;
+
+    for (long long row = first; row < a.rows; row += step) {
+        const T *x = a.x + row * a.x_stride;
+        const T *r = a.r ? a.r + row * a.r_stride : nullptr;
+        float s[CH][V];
+        Pack<T, V> px[CH], pr[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * lanes + lane) * V;
+            if (at < a.width) {
+                px[c] = *reinterpret_cast<const Pack<T, V> *>(x + at);
+                if (r) pr[c] = *reinterpret_cast<const Pack<T, V> *>(r + at);
+            }
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const bool in = (c * lanes + lane) * V < a.width;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float f = in ? to_float(px[c].v[i]) : 0.f;
+                if (r && in) f = fmaf(a.alpha, to_float(pr[c].v[i]), f);
+                s[c][i] = f;
+                sum += f;
+            }
+        }
+        float mean = 0.f, factor = 1.f;
+        if (a.kind != OPENFISH_B200_NORM_NONE) {
+            if (a.kind == OPENFISH_B200_NORM_LAYER) mean = reduce<BLOCK>(sum, scratch, add) * inv;
+            float sq = 0.f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const bool in = (c * lanes + lane) * V < a.width;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = s[c][i] - mean;
+                    if (in) sq = fmaf(d, d, sq);
+                }
+            }
+            factor = 1.f / sqrtf(reduce<BLOCK>(sq, scratch, add) * inv + a.eps);
+        }
+        float top = 0.f;
+        bool odd = false;  // an infinity or NaN in the row
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * lanes + lane) * V;
+            if (at < a.width) {
+                if (a.kind != OPENFISH_B200_NORM_NONE) {
+                    Pack<T, V> w, b;
+                    if (a.w) w = *reinterpret_cast<const Pack<T, V> *>(a.w + at);
+                    if (a.b) b = *reinterpret_cast<const Pack<T, V> *>(a.b + at);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        float y = (s[c][i] - mean) * factor;
+                        if (a.w) y *= to_float(w.v[i]);
+                        if (a.b) y += to_float(b.v[i]);
+                        s[c][i] = y;
+                    }
+                }
+                if (a.out) {
+                    Pack<T, V> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(s[c][i]);
+                    *reinterpret_cast<Pack<T, V> *>(a.out + row * a.out_stride + at) = o;
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    top = fmaxf(top, fabsf(s[c][i]));
+                    odd |= !(fabsf(s[c][i]) < INFINITY);
+                }
+            }
+        }
+        if (!a.q) continue;
+        // (fmaxf drops a NaN; such a row counts as one with an infinity)
+        top = reduce<BLOCK>(odd ? INFINITY : top, scratch, most);
+        const bool fine = top < INFINITY;
+        const float scale = top / 127.f;
+        // y * (127 / top) may miss y / scale by an ulp, which moves a value that lies on the border of two steps.  A
+        // top so small that 127 / top overflows is divided by.
+        const float back = 127.f / top;
+        const bool direct = back < INFINITY;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * lanes + lane) * V;
+            if (at < a.width) {
+                Pack8<V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float f = !fine || top == 0.f ? 0.f : direct ? s[c][i] * back : s[c][i] / top * 127.f;
+                    o.v[i] = (int8_t)max(-127, min(127, __float2int_rn(f)));
+                }
+                *reinterpret_cast<Pack8<V> *>(a.q + row * a.q_stride + at) = o;
+            }
+        }
+        if (lane == 0) a.q_scale[row] = fine ? scale : NAN;
+    }
+}
+
+template <class T, int V, int CH, bool BLOCK>
+void launch(const NormArgs<T> &a, int threads, int sms, cudaStream_t stream) {
+    const long long per_block = BLOCK ? 1 : threads / 32;
+    long long blocks = (a.rows + per_block - 1) / per_block;
+    const long long cap = (long long)sms * (2048 / threads) * 4;
+    if (blocks > cap) blocks = cap;
+    norm_kernel<T, V, CH, BLOCK><<<(unsigned)blocks, threads, 0, stream>>>(a);
+}
+
+// A warp to a row while 4 packs (of one element: 16) to a lane hold it, else a block with as few packs to a thread as 1024
+// threads allow.
+template <class T, int V>
+void dispatch(const NormArgs<T> &a, int sms, cudaStream_t stream) {
+    const int packs = (a.width + V - 1) / V;
+    constexpr int S = V == 8 ? 1 : 4;  // scalar packs are an eighth of the size: more of them
+    if (packs <= 32 * S) launch<T, V, S, false>(a, 128, sms, stream);
+    else if (packs <= 64 * S) launch<T, V, 2 * S, false>(a, 128, sms, stream);
+    else if (packs <= 128 * S) launch<T, V, 4 * S, false>(a, 128, sms, stream);
+    else if (packs <= 1024 * S) launch<T, V, S, true>(a, ((packs + S - 1) / S + 31) / 32 * 32, sms, stream);
+    else launch<T, V, 4 * (8 / V), true>(a, 1024, sms, stream);
+}
+
+template <class T>
+int run(cudaStream_t stream, const openfish_b200_norm_t *p, int sms) {
+    NormArgs<T> a;
+    a.x = static_cast<const T *>(p->x); a.r = static_cast<const T *>(p->residual);
+    a.w = static_cast<const T *>(p->weight); a.b = static_cast<const T *>(p->bias);
+    a.out = static_cast<T *>(p->out); a.q = p->q; a.q_scale = p->q_scale;
+    a.x_stride = p->x_stride; a.r_stride = p->residual_stride; a.out_stride = p->out_stride; a.q_stride = p->q_stride;
+    a.rows = p->rows; a.width = p->width; a.kind = p->kind; a.eps = p->eps; a.alpha = p->residual_scale;
+    const auto fits = [&](const void *q, long long stride, int to) {
+        return !q || ((uintptr_t)q % to == 0 && (p->rows == 1 || stride % 8 == 0));
+    };
+    if (p->width % 8 == 0 && fits(p->x, p->x_stride, 16) && fits(p->residual, p->residual_stride, 16) && fits(p->weight, 0, 16) &&
+        fits(p->bias, 0, 16) && fits(p->out, p->out_stride, 16) && fits(p->q, p->q_stride, 8))
+        dispatch<T, 8>(a, sms, stream);
+    else
+        dispatch<T, 1>(a, sms, stream);
+    return ofe::launched();
+}
+
+}  // namespace
+
+extern "C" int ofb_norm(void *stream, const openfish_b200_norm_t *a) {
+    int sms = 0;
+    if (const int rc = ofe::sm_count(&sms)) return rc;
+    return a->dtype == OPENFISH_B200_F16 ? run<__half>((cudaStream_t)stream, a, sms) : run<__nv_bfloat16>((cudaStream_t)stream, a, sms);
+}

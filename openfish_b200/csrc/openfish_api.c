@@ -9,6 +9,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "api_util.h"
 #include "backend.h"
 #include "openfish_b200.h"
 
@@ -52,6 +53,11 @@ static int backend_failed(const char *func, int rc) {
     raise_error(func, rc, ofb_error_text());
     return 1;
 }
+
+/* The same for the entry points of other files (api_util.h). */
+void ofb_api_raise(const char *func, int code, const char *text) { raise_error(func, code, text); }
+void ofb_api_clear(void) { clear_error(); }
+int ofb_api_backend_failed(const char *func, int rc) { return backend_failed(func, rc); }
 
 static int states_of(int state_len) { return 1 << (2 * state_len); }
 
