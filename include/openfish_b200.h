@@ -242,8 +242,8 @@ void openfish_b200_attention(void *cuda_stream, const openfish_b200_attention_t 
  *
  *   out[m][n] = x_scale[m] * w_scale[n] * sum_k x[m][k] * w[n][k]  (+ bias[n])
  *
- * The sum is exact.  x [rows][depth], w [cols][depth] int8, each row on a 16-byte boundary (strides multiples of 16; what
- * lies between depth and the stride is not used); depth up to 131071 (beyond, the sum could leave 32 bits).  x_scale [rows],
+ * The sum is exact.  x [rows][depth], w [cols][depth] int8, each row on a 16-byte boundary (strides multiples of 16; a row
+ * may be read up to the next such boundary, what lies there is not used); depth up to 131071 (beyond, the sum could leave 32 bits).  x_scale [rows],
  * w_scale [cols] fp32; bias [cols] or NULL and out [rows][cols] of type `dtype`. */
 typedef struct openfish_b200_matmul_i8 {
     int dtype; /* of out and bias */

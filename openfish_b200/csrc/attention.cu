@@ -76,9 +76,4 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *a) {
     return ofe::launched();
 }
 
-extern "C" int ofb_encoder_wait(void *stream) {
-    if (const int rc = ofe::cuda_status(cudaStreamSynchronize((cudaStream_t)stream))) return rc;
-    int status = 0;
-    if (const int rc = ofe::cuda_status(cudaMemcpyFromSymbol(&status, g_status, sizeof(status)))) return rc;
-    return OPENFISH_B200_OK;
-}
+extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }

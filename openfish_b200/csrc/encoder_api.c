@@ -177,6 +177,10 @@ void openfish_b200_norm(void *cuda_stream, const openfish_b200_norm_t *a) {
 }
 
 void openfish_b200_encoder_wait(void *cuda_stream) {
+    int a = 0, m = 0;
     ofb_api_clear();
-    ofb_api_backend_failed(__func__, ofb_encoder_wait(cuda_stream));
+    if (ofb_api_backend_failed(__func__, ofb_attention_settle(cuda_stream, &a)) ||
+        ofb_api_backend_failed(__func__, ofb_matmul_i8_settle(cuda_stream, &m)))
+        return;
+    if (a || m) refuse(__func__, OPENFISH_B200_ERR_DEVICE_WAIT, "a kernel gave up waiting; results queued since the last such call are meaningless");
 }

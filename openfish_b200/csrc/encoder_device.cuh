@@ -26,5 +26,18 @@ inline int sm_count(int *out) {
     if (const int rc = cuda_status(cudaGetDevice(&dev))) return rc;
     return cuda_status(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
 }
+// Waits for the stream, then reads a file's status word and clears it.
+inline int settle(cudaStream_t stream, const int &symbol, int *gave_up) {
+    int seen = 0;
+    const int none = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&seen, symbol, sizeof(seen), 0, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e == cudaSuccess && seen) {
+        e = cudaMemcpyToSymbolAsync(symbol, &none, sizeof(none), 0, cudaMemcpyHostToDevice, stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    }
+    *gave_up = seen != 0;
+    return cuda_status(e);
+}
 
 }  // namespace ofe

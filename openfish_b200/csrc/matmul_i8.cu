@@ -1,52 +1,349 @@
 // matmul_i8.cu -- product of tokens and weights in 8-bit integers (openfish_b200_matmul_i8).
 //
 //   out[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]
+//
+// A handful of tokens reads the weights once and is bound by that: matmul_few_kernel, four products to an
+// instruction.  Anything else goes to the matrix instructions: matmul_tile_kernel.
 #include <stdint.h>
 
 #include "encoder_device.cuh"
+#include "tc5.cuh"
 
 namespace {
 
-constexpr int kTile = 64, kDepth = 64;
+__device__ int g_status;  // of the kernels on this device: a wait that ran out
+
+struct Args {
+    const int8_t *x, *w;
+    const float *x_scale, *w_scale;
+    const void *bias;
+    void *out;
+    long long x_stride, w_stride, out_stride;
+    int rows, cols, depth;
+    bool by_copy;  // out goes through the tiled copies
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// Tiles of 128 * CG tokens by BN channels.  CG = 2: a pair of blocks on two neighbouring SMs shares one tile, each holding half of
+// the tokens and half of the channels' weights, so that a byte of shared memory is filled once and read by both.
+//
+// Warps: 0 issues the copies, 1 the matrix instructions, 4 to 7 (a quarter of the accumulator's 128 lanes each) scale and
+// store.  The accumulator is there twice, so that one tile's sums are stored while the next one's are formed.
+template <int CG, int BN>
+struct Shape {
+    static constexpr int kRowsB = BN / CG;                     // weights' rows in one block
+    static constexpr int kStageBytes = (128 + kRowsB) * 128;   // 128 deep
+    static constexpr int kStages = BN == 64 ? 7 : 5;
+    static constexpr int kOutBytes = 4 * 2 * 4096;             // a warp's 32 rows of 64 results, twice
+    static constexpr int kScaleBytes = 4 * 64 * 8;             // a warp's 64 channel scales and biases
+    static constexpr int kBytes = 1024 + kStages * kStageBytes + kOutBytes + kScaleBytes + (2 * kStages + 5) * 8 + 8;
+    static constexpr int kColumns = 2 * BN;                    // of tensor memory, a power of two
+};
+
+struct Walk {  // the tiles in the order in which they are taken: stripes of 8 tiles of tokens, through all channels each
+    int tiles_m, tiles_n;
+    __device__ __forceinline__ void at(int t, int *m, int *n) const {
+        const int stripe = t / (8 * tiles_n), first = stripe * 8;
+        const int high = min(8, tiles_m - first), in = t - stripe * 8 * tiles_n;
+        *m = first + in % high;
+        *n = in / high;
+    }
+};
+
+template <class T, int CG, int BN>
+__global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
+                                                           const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
+    using S = Shape<CG, BN>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *const base = raw + ((1024 - (tc5::smem_u32(raw) & 1023)) & 1023);
+    uint8_t *const out_stage = base + S::kStages * S::kStageBytes;
+    float2 *const scale_stage = reinterpret_cast<float2 *>(out_stage + S::kOutBytes);
+    uint64_t *const full = reinterpret_cast<uint64_t *>(out_stage + S::kOutBytes + S::kScaleBytes);
+    uint64_t *const empty = full + S::kStages, *const sum_full = empty + S::kStages, *const sum_empty = sum_full + 2, *const done = sum_empty + 2;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CG == 2 ? blockIdx.x & 1 : 0;
+    const int group = blockIdx.x / CG, groups = gridDim.x / CG;
+    const Walk walk{(a.rows + 128 * CG - 1) / (128 * CG), (a.cols + BN - 1) / BN};
+    const int tiles = walk.tiles_m * walk.tiles_n;
+    const int steps = (a.depth + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        *given_up = 0;
+        for (int i = 0; i < S::kStages; ++i) {
+            ofd::mbar_init(&full[i], 1);
+            ofd::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ofd::mbar_init(&sum_full[i], 1);
+            ofd::mbar_init(&sum_empty[i], 4 * CG);
+        }
+        ofd::mbar_init(done, 1);
+        ofd::mbar_fence_init();
+        tc5::prefetch_map(&map_x);
+        tc5::prefetch_map(&map_w);
+    }
+    if (warp == 1) tc5::tmem_alloc<CG>(tmem_slot, S::kColumns);
+    tc5::before_sync();
+    __syncthreads();
+    if (CG == 2) tc5::cluster_sync();
+    tc5::after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        // copies: each block its own rows; the bytes of both are counted at the first block's barrier
+        int i = 0;
+        bool fine = true;
+        for (int t = group; t < tiles && fine; t += groups) {
+            int tm, tn;
+            walk.at(t, &tm, &tn);
+            const int m = tm * 128 * CG + rank * 128, n = tn * BN + rank * S::kRowsB;
+            for (int k = 0; k < steps; ++k, ++i) {
+                const int s = i % S::kStages;
+                fine = tc5::wait(&empty[s], ((i / S::kStages) & 1) ^ 1, given_up, &g_status);
+                if (!fine) break;
+                uint8_t *const to = base + s * S::kStageBytes;
+                if (CG == 1) {
+                    ofd::mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+                    tc5::load_2d(to, &map_x, k * 128, m, &full[s]);
+                    tc5::load_2d(to + 128 * 128, &map_w, k * 128, n, &full[s]);
+                } else {
+                    if (rank == 0) ofd::mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);
+                    const uint32_t bar = tc5::of_first_block(tc5::smem_u32(&full[s]));
+                    tc5::load_2d_pair(to, &map_x, k * 128, m, bar);
+                    tc5::load_2d_pair(to + 128 * 128, &map_w, k * 128, n, bar);
+                }
+            }
+        }
+        // after a wait that ran out: the copies under way land before the block ends
+        if (!fine && rank == 0) ofd::mbar_drain_bounded(full, S::kStages, i, ofd::kDefaultWaitLimitNs);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = tc5::idesc_i8(128 * CG, BN);
+        int i = 0, j = 0;
+        bool fine = true;
+        for (int t = group; t < tiles && fine; t += groups, ++j) {
+            const uint32_t sum = tmem + (j & 1) * BN;
+            fine = tc5::wait(&sum_empty[j & 1], ((j >> 1) & 1) ^ 1, given_up, &g_status);
+            if (!fine) break;
+            tc5::after_sync();
+            for (int k = 0; k < steps; ++k, ++i) {
+                const int s = i % S::kStages;
+                fine = tc5::wait(&full[s], (i / S::kStages) & 1, given_up, &g_status);
+                if (!fine) break;
+                tc5::after_sync();
+                const uint32_t at = tc5::smem_u32(base + s * S::kStageBytes);
+                const uint64_t da = tc5::desc_k_major(at), db = tc5::desc_k_major(at + 128 * 128);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tc5::mma_i8<CG>(sum, da + 2 * q, db + 2 * q, idesc, (k | q) != 0);
+                if (CG == 1) tc5::commit(&empty[s]);
+                else tc5::commit_pair(&empty[s]);
+            }
+            if (!fine) break;
+            if (CG == 1) tc5::commit(&sum_full[j & 1]);
+            else tc5::commit_pair(&sum_full[j & 1]);
+        }
+        if (!fine) {  // after a wait that ran out: the instructions under way end before the block does
+            if (CG == 1) tc5::commit(done);
+            else tc5::commit_pair(done);
+            ofd::mbar_land(done, 0, 0, ofd::kDefaultWaitLimitNs);
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3;
+        uint8_t *const mine = out_stage + quarter * 8192;
+        float2 *const scales = scale_stage + quarter * 64;
+        const T *const bias = static_cast<const T *>(a.bias);
+        int j = 0, turn = 0;
+        for (int t = group; t < tiles; t += groups, ++j) {
+            int tm, tn;
+            walk.at(t, &tm, &tn);
+            const int m0 = tm * 128 * CG + rank * 128 + quarter * 32, n0 = tn * BN;
+            const float xs = m0 + lane < a.rows ? a.x_scale[m0 + lane] : 0.f;
+            const bool fine = tc5::wait(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status);
+            if (__any_sync(0xffffffffu, !fine)) break;
+            tc5::after_sync();
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 64, ++turn) {
+                const uint32_t sum = tmem + ((uint32_t)(quarter * 32) << 16) + (j & 1) * BN + c;
+                uint32_t v[2][32];
+                tc5::ld32(v[0], sum);
+                tc5::ld32(v[1], sum + 32);
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int n = n0 + c + h * 32 + lane;
+                    float2 sb = {0.f, 0.f};
+                    if (n < a.cols) {
+                        sb.x = a.w_scale[n];
+                        if (bias) sb.y = ofe::to_float(bias[n]);
+                    }
+                    scales[h * 32 + lane] = sb;
+                }
+                if (lane == 0) tc5::store_wait_read<1>();  // the copy out of this half of the staging memory is done with it
+                __syncwarp();
+                tc5::ld_wait(v[0]);
+                tc5::ld_wait(v[1]);
+                if (c + 64 >= BN) {  // the accumulator has been read: the next tile's sums may go there
+                    tc5::before_sync();
+                    if (lane == 0) {
+                        if (CG == 1) tc5::arrive(&sum_empty[j & 1]);
+                        else tc5::arrive_cluster(tc5::of_first_block(tc5::smem_u32(&sum_empty[j & 1])));
+                    }
+                }
+                uint8_t *const to = mine + (turn & 1) * 4096;
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    alignas(16) T o[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float4 sb = reinterpret_cast<const float4 *>(scales)[p * 4 + e / 2];
+                        const int at = (p & 3) * 8 + e;
+                        o[e] = ofe::from_float<T>(fmaf((float)(int)v[p >> 2][at], xs * sb.x, sb.y));
+                        o[e + 1] = ofe::from_float<T>(fmaf((float)(int)v[p >> 2][at + 1], xs * sb.z, sb.w));
+                    }
+                    *reinterpret_cast<uint4 *>(to + lane * 128 + ((p ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(o);
+                }
+                if (a.by_copy) {
+                    tc5::fence_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (n0 + c < a.cols && m0 < a.rows) tc5::store_2d(&map_out, n0 + c, m0, to);
+                        tc5::store_commit();
+                    }
+                } else {
+                    // rows of out that start anywhere: two results to a lane, a row to an instruction
+                    __syncwarp();
+                    T *const out = static_cast<T *>(a.out) + (long long)m0 * a.out_stride + n0 + c;
+                    for (int r = 0; r < 32 && m0 + r < a.rows; ++r) {
+                        const T *const from = reinterpret_cast<const T *>(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4)) + (lane & 3) * 2;
+                        if (n0 + c + 2 * lane < a.cols) out[r * a.out_stride + 2 * lane] = from[0];
+                        if (n0 + c + 2 * lane + 1 < a.cols) out[r * a.out_stride + 2 * lane + 1] = from[1];
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) tc5::store_wait_read<0>();
+    }
+    __syncwarp();
+    tc5::before_sync();
+    __syncthreads();
+    if (CG == 2) tc5::cluster_sync();
+    tc5::after_sync();
+    if (warp == 1) tc5::tmem_free<CG>(tmem, S::kColumns);
+}
+
+template <class T, int CG, int BN>
+int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
+    using S = Shape<CG, BN>;
+    CUtensorMap mx, mw, mo;
+    const auto map8 = [](CUtensorMap *map, const int8_t *base, int rows, int depth, long long stride, int box_rows) {
+        const cuuint64_t dims[2] = {(cuuint64_t)depth, (cuuint64_t)rows};
+        const cuuint64_t strides[1] = {rows > 1 ? (cuuint64_t)stride : (cuuint64_t)((depth + 15) / 16 * 16)};
+        const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+        return tc5::make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
+    };
+    bool made = map8(&mx, a.x, a.rows, a.depth, a.x_stride, 128) && map8(&mw, a.w, a.cols, a.depth, a.w_stride, S::kRowsB);
+    if (made && a.by_copy) {
+        const cuuint64_t dims[2] = {(cuuint64_t)a.cols, (cuuint64_t)a.rows};
+        const cuuint64_t strides[1] = {(cuuint64_t)(a.rows > 1 ? a.out_stride : (a.cols + 7) / 8 * 8) * 2};
+        const cuuint32_t box[2] = {64, 32};
+        made = tc5::make_map(&mo, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a.out, dims, strides, box);
+    } else {
+        mo = mw;
+    }
+    if (!made) return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
+    const auto kernel = matmul_tile_kernel<T, CG, BN>;
+    if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
+    const long long tiles = ((long long)(a.rows + 128 * CG - 1) / (128 * CG)) * ((a.cols + BN - 1) / BN);
+    const int most = sms / CG;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = S::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CG > 1 ? 1 : 0;
+    return ofe::cuda_status(cudaLaunchKernelEx(&cfg, kernel, a, mx, mw, mo));
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// A few tokens: a warp to a channel, its lanes 16 bytes of the weights each at a time; the tokens come from the cache.
+template <class T, int MT>
+__global__ void __launch_bounds__(128) matmul_few_kernel(const Args a) {
+    const int lane = threadIdx.x & 31;
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 5), m0 = blockIdx.y * MT;
+    if (n >= a.cols) return;
+    int sum[MT] = {};
+    const int8_t *const w = a.w + (long long)n * a.w_stride;
+#pragma unroll 4
+    for (int k = lane * 16; k < a.depth; k += 512) {
+        int4 wv = *reinterpret_cast<const int4 *>(w + k);
+        if (k + 16 > a.depth) {  // what lies behind the row is no part of it
+            int *const word = reinterpret_cast<int *>(&wv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int keep = a.depth - k - 4 * i;  // bytes of this word
+                word[i] = keep >= 4 ? word[i] : keep <= 0 ? 0 : word[i] & ((1 << (8 * keep)) - 1);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if (m0 + i < a.rows) {
+                const int4 xv = *reinterpret_cast<const int4 *>(a.x + (m0 + i) * a.x_stride + k);
+                sum[i] = __dp4a(xv.x, wv.x, sum[i]);
+                sum[i] = __dp4a(xv.y, wv.y, sum[i]);
+                sum[i] = __dp4a(xv.z, wv.z, sum[i]);
+                sum[i] = __dp4a(xv.w, wv.w, sum[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int s = __reduce_add_sync(0xffffffffu, sum[i]);
+        if (lane == i && m0 + i < a.rows) {
+            const float b = a.bias ? ofe::to_float(static_cast<const T *>(a.bias)[n]) : 0.f;
+            static_cast<T *>(a.out)[(m0 + i) * a.out_stride + n] = ofe::from_float<T>(fmaf((float)s, a.x_scale[m0 + i] * a.w_scale[n], b));
+        }
+    }
+}
+
+template <class T, int MT>
+int launch_few(const Args &a, cudaStream_t stream) {
+    matmul_few_kernel<T, MT><<<dim3((unsigned)((a.cols + 3) / 4), (unsigned)((a.rows + MT - 1) / MT)), 128, 0, stream>>>(a);
+    return ofe::launched();
+}
 
 template <class T>
-__global__ void __launch_bounds__(256) matmul_simple_kernel(const openfish_b200_matmul_i8_t a) {
-    __shared__ int sx[kTile][kDepth / 4 + 1], sw[kTile][kDepth / 4 + 1];
-    const long long m0 = (long long)blockIdx.x * kTile;
-    const int n0 = blockIdx.y * kTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < a.depth; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-            const int row = i / kDepth, k = i % kDepth;
-            const bool in = k0 + k < a.depth;
-            reinterpret_cast<int8_t *>(&sx[row][0])[k] = in && m0 + row < a.rows ? a.x[(m0 + row) * a.x_stride + k0 + k] : 0;
-            reinterpret_cast<int8_t *>(&sw[row][0])[k] = in && n0 + row < a.cols ? a.w[(n0 + row) * a.w_stride + k0 + k] : 0;
-        }
-        __syncthreads();
-        for (int k = 0; k < kDepth / 4; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sx[ty * 4 + i][k], sw[tx * 4 + j][k], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const long long m = m0 + ty * 4 + i;
-            const int n = n0 + tx * 4 + j;
-            if (m >= a.rows || n >= a.cols) continue;
-            float y = (float)acc[i][j] * (a.x_scale[m] * a.w_scale[n]);
-            if (a.bias) y += ofe::to_float(static_cast<const T *>(a.bias)[n]);
-            static_cast<T *>(a.out)[m * a.out_stride + n] = ofe::from_float<T>(y);
-        }
+int run(const Args &a, int sms, cudaStream_t stream) {
+    if (a.rows <= 1) return launch_few<T, 1>(a, stream);
+    if (a.rows <= 2) return launch_few<T, 2>(a, stream);
+    if (a.rows <= 4) return launch_few<T, 4>(a, stream);
+    if (a.rows <= 8) return launch_few<T, 8>(a, stream);
+    const long long tiles_m = (a.rows + 127) / 128;
+    if (tiles_m * ((a.cols + 127) / 128) <= sms) return launch_tiles<T, 1, 64>(a, sms, stream);
+    if (((tiles_m + 1) / 2) * ((a.cols + 255) / 256) * 2 <= sms) return launch_tiles<T, 1, 128>(a, sms, stream);
+    return launch_tiles<T, 2, 256>(a, sms, stream);
 }
 
 }  // namespace
 
 extern "C" size_t ofb_matmul_i8_workspace(const openfish_b200_matmul_i8_t *) { return 0; }
 
-extern "C" int ofb_matmul_i8(void *stream, const openfish_b200_matmul_i8_t *a) {
-    const dim3 grid((unsigned)((a->rows + kTile - 1) / kTile), (unsigned)((a->cols + kTile - 1) / kTile));
-    if (a->dtype == OPENFISH_B200_F16) matmul_simple_kernel<__half><<<grid, 256, 0, (cudaStream_t)stream>>>(*a);
-    else matmul_simple_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>(*a);
-    return ofe::launched();
+extern "C" int ofb_matmul_i8(void *stream, const openfish_b200_matmul_i8_t *p) {
+    int sms = 0;
+    if (const int rc = ofe::sm_count(&sms)) return rc;
+    Args a;
+    a.x = p->x; a.w = p->w; a.x_scale = p->x_scale; a.w_scale = p->w_scale; a.bias = p->bias; a.out = p->out;
+    a.x_stride = p->x_stride; a.w_stride = p->w_stride; a.out_stride = p->out_stride;
+    a.rows = (int)p->rows; a.cols = p->cols; a.depth = p->depth;
+    a.by_copy = (uintptr_t)p->out % 16 == 0 && (p->rows == 1 || p->out_stride % 8 == 0);
+    return p->dtype == OPENFISH_B200_F16 ? run<__half>(a, sms, (cudaStream_t)stream) : run<__nv_bfloat16>(a, sms, (cudaStream_t)stream);
 }
+
+extern "C" int ofb_matmul_i8_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }
