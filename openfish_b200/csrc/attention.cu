@@ -1,79 +1,564 @@
 // attention.cu -- attention over packed sequences (openfish_b200_attention).
+//
+//   out[i] = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(c <q_i, k_j> - m_i),   c = scale log2(e),
+//
+// in one pass over the keys: m_i is a running maximum, and what has been summed is scaled when it moves.
+//
+// A block takes 256 rows of one sequence and key head.  The query heads that share a key head are rows next to each
+// other (row r is query r / g, head r % g of the group), so that grouped heads and single tokens fill the same tiles and
+// a key is read once for all of them.  The rows are two halves of 128, and the keys come in tiles of 128:
+//
+//   warps 0-3, 4-7   the softmax of the first and second half, a thread to a row
+//   warp 8           asynchronous copies of the keys' and values' tiles into a ring in shared memory
+//   warp 9           matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there
+//
+// P takes the place of the S it came from.  While one half's weights are worked out, the matrix unit is busy with the other
+// half's: O += P V of the last tile, then S of the next one.
 #include <math.h>
 #include <stdint.h>
 
 #include "encoder_device.cuh"
+#include "tc5.cuh"
 
 namespace {
 
-// A sequence's rows in a tensor of `rows`, cut to the room there is.
-__device__ __forceinline__ void span(const int32_t *start, const int32_t *used, int s, long long rows, int most, int *first, int *count) {
-    const long long lo = min(max((long long)start[s], 0LL), rows), hi = min(max((long long)start[s + 1], lo), rows);
-    long long n = hi - lo;
-    if (used) n = min(n, max((long long)used[s], 0LL));
-    *first = (int)lo;
-    *count = (int)min(n, (long long)most);
-}
-
-// A warp to a query and head: 32 keys at a time, a lane to a key for the scores, a lane to four elements for the sum.
-template <class T>
-__global__ void __launch_bounds__(128) attention_simple_kernel(const openfish_b200_attention_t a) {
-    const int lane = threadIdx.x & 31;
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int i = (int)(at / a.q_heads), h = (int)(at % a.q_heads);
-    for (int s = blockIdx.y; s < a.sequences; s += gridDim.y) {
-    int q0, nq, k0, nk;
-    span(a.q_start, a.q_used, s, a.q_rows, a.max_q, &q0, &nq);
-    span(a.k_start, a.k_used, s, a.k_rows, a.max_k, &k0, &nk);
-    if (i >= nq) continue;
-    const int kh = h / (a.q_heads / a.kv_heads);
-    const T *q = static_cast<const T *>(a.q) + (long long)(q0 + i) * a.q_stride_row + h * a.q_stride_head;
-    const T *k = static_cast<const T *>(a.k) + (long long)k0 * a.k_stride_row + kh * a.k_stride_head;
-    const T *v = static_cast<const T *>(a.v) + (long long)k0 * a.v_stride_row + kh * a.v_stride_head;
-    T *o = static_cast<T *>(a.out) + (long long)(q0 + i) * a.out_stride_row + h * a.out_stride_head;
-    const int place = i + nk - nq;
-    const int lo = a.window_left < 0 ? 0 : (int)max((long long)place - a.window_left, 0LL);
-    const int hi = a.window_right < 0 ? nk : (int)min((long long)place + a.window_right + 1, (long long)nk);
-    float top = -INFINITY, total = 0.f, acc[4] = {};
-    for (int j0 = lo; j0 < hi; j0 += 32) {
-        const int j = j0 + lane;
-        float z = -INFINITY;
-        if (j < hi) {
-            z = 0.f;
-            for (int d = 0; d < a.head_dim; ++d) z = fmaf(ofe::to_float(q[d]), ofe::to_float(k[(long long)j * a.k_stride_row + d]), z);
-            z *= a.scale;
-        }
-        float m = z;
-        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        m = fmaxf(m, top);
-        const float fade = top == m ? 1.f : expf(top - m), p = j < hi ? expf(z - (m == -INFINITY ? 0.f : m)) : 0.f;
-        top = m;
-        float t = p;
-        for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-        total = total * fade + t;
-        for (int c = 0; c < 4; ++c) acc[c] *= fade;
-        for (int n = 0; n < 32 && j0 + n < hi; ++n) {
-            const float pn = __shfl_sync(0xffffffffu, p, n);
-            for (int c = 0; c < 4; ++c)
-                if (c * 32 + lane < a.head_dim) acc[c] = fmaf(pn, ofe::to_float(v[(long long)(j0 + n) * a.v_stride_row + c * 32 + lane]), acc[c]);
-        }
-    }
-    for (int c = 0; c < 4; ++c)
-        if (c * 32 + lane < a.head_dim) o[c * 32 + lane] = ofe::from_float<T>(hi > lo ? acc[c] / total : 0.f);
-    }
-}
-
 __device__ int g_status;  // of the kernels on this device: a wait that ran out
+
+constexpr int kHalf = 128;  // rows of a half
+constexpr int kKeys = 128;  // keys of a tile
+constexpr int kThreads = 320;
+constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled: weights up to 256
+
+struct Args {
+    const int32_t *q_start, *k_start, *q_used, *k_used;
+    const void *q, *k, *v;
+    void *out;
+    float *part, *part_lse;  // of a split: [split][q_rows][q_heads][head_dim] and [split][q_rows][q_heads]
+    long long q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head, out_stride_row, out_stride_head;
+    int q_rows, k_rows, q_heads, kv_heads, group, head_dim, sequences, max_q, max_k, left, right;
+    int tiles, splits;  // of 256 rows of the longest sequence; pieces of a tile's keys
+    float c;
+};
+
+// A sequence's rows in a tensor of `rows`, cut to the room there is.
+__device__ __forceinline__ void span(const int32_t *start, const int32_t *used, int s, int rows, int most, int *first, int *count) {
+    const int lo = min(max(start[s], 0), rows), hi = min(max(start[s + 1], lo), rows);
+    int n = hi - lo;
+    if (used) n = min(n, max(used[s], 0));
+    *first = lo;
+    *count = min(n, most);
+}
+// The keys that query i of nq sees of nk: [lo, hi).
+__device__ __forceinline__ void window(const Args &a, int i, int nq, int nk, int *lo, int *hi) {
+    const int place = i + nk - nq;
+    *lo = a.left < 0 ? 0 : max(place - a.left, 0);
+    *hi = a.right < 0 ? nk : min(place + a.right + 1, nk);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <int DP>
+struct Shape {
+    static constexpr int kChunks = DP / 64;                   // of 64 elements, 128 bytes
+    static constexpr int kTileBytes = kChunks * 128 * 128;    // 128 rows
+    static constexpr int kStages = DP == 64 ? 10 : 5;
+    static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes + (2 * kStages + 8) * 8 + 16;
+    static constexpr int kOut = 256;                          // the sums' first column of tensor memory, behind two S
+};
+
+// One row again, by a warp, straight from its definition and reading only the keys that the row sees.  A matrix
+// instruction multiplies the values of masked keys by weights of zero, which is no zero where such a value is an infinity or NaN.
+template <class T>
+__device__ __noinline__ float2 redo_row(const T *q, const T *k, const T *v, long long k_stride, long long v_stride, int head_dim, float c, int lo,
+                                        int hi, float *out, T *out16) {
+    const int lane = threadIdx.x & 31;
+    float qf[4], acc[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        qf[n] = lane + 32 * n < head_dim ? ofe::to_float(q[lane + 32 * n]) : 0.f;
+        acc[n] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    for (int j = lo; j < hi && l == l; ++j) {
+        float z = 0.f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (lane + 32 * n < head_dim) z = fmaf(qf[n], ofe::to_float(k[j * k_stride + lane + 32 * n]), z);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+        const float next = fmaxf(m, z), from = next == -INFINITY ? 0.f : next;
+        const float fade = m == next ? 1.f : ex2((m - next) * c), p = ex2((z - from) * c);
+        m = next;
+        l = l * fade + p;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (lane + 32 * n < head_dim) acc[n] = fmaf(p, ofe::to_float(v[j * v_stride + lane + 32 * n]), acc[n] * fade);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int d = lane + 32 * n;
+        if (d >= head_dim) continue;
+        // a sum that is no number makes every element none (the loop ends there)
+        const float f = l == l ? acc[n] / l : NAN;
+        if (out16) out16[d] = ofe::from_float<T>(f);
+        else out[d] = f;
+    }
+    return make_float2(m, l);
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
+                                                                const __grid_constant__ CUtensorMap map_v) {
+    using S = Shape<DP>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- which rows, which keys.  The last rows come first: under a causal mask they have the most keys.
+    const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
+    const int pairs = a.kv_heads * a.sequences;
+    const int kh = rest % pairs % a.kv_heads, seq = rest % pairs / a.kv_heads, tile = a.tiles - 1 - rest / pairs;
+    int q0, nq, k0, nk;
+    span(a.q_start, a.q_used, seq, a.q_rows, a.max_q, &q0, &nq);
+    span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
+    const int rows = nq * a.group, r0 = tile * 2 * kHalf;
+    if (r0 >= rows) return;
+    int lo[2], hi[2];  // the keys that a half's rows see between them
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int first = r0 + x * kHalf, last = min(first + kHalf, rows) - 1;
+        lo[x] = hi[x] = 0;
+        if (first < rows) {
+            int unused;
+            window(a, first / a.group, nq, nk, &lo[x], &unused);
+            window(a, last / a.group, nq, nk, &unused, &hi[x]);
+            if (hi[x] <= lo[x]) lo[x] = hi[x] = 0;
+        }
+    }
+    const int base = hi[1] <= lo[1] ? lo[0] : hi[0] <= lo[0] ? lo[1] : min(lo[0], lo[1]);
+    const int tiles = (max(max(hi[0], hi[1]) - base, 0) + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
+    int from[2], to[2];  // each half's tiles
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        from[x] = to[x] = 0;
+        if (hi[x] > lo[x]) {
+            from[x] = max(t0, (lo[x] - base) / kKeys);
+            to[x] = min(t1, (hi[x] - base + kKeys - 1) / kKeys);
+            if (to[x] <= from[x]) from[x] = to[x] = 0;
+        }
+    }
+
+    extern __shared__ uint8_t raw[];
+    uint8_t *const q_tiles = raw + ((1024 - (tc5::smem_u32(raw) & 1023)) & 1023);
+    uint8_t *const ring = q_tiles + 2 * S::kTileBytes;
+    uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kTileBytes), *const empty = full + S::kStages;
+    uint64_t *const q_ready = empty + S::kStages, *const s_full = q_ready + 2, *const p_ready = s_full + 2, *const o_full = p_ready + 2;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+    volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    if (threadIdx.x == 0) {
+        *given_up = 0;
+        for (int i = 0; i < S::kStages; ++i) {
+            ofd::mbar_init(&full[i], 1);
+            ofd::mbar_init(&empty[i], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            ofd::mbar_init(&q_ready[x], 4);
+            ofd::mbar_init(&s_full[x], 1);
+            ofd::mbar_init(&p_ready[x], 4);
+            ofd::mbar_init(&o_full[x], 1);
+        }
+        ofd::mbar_fence_init();
+        tc5::prefetch_map(&map_k);
+        tc5::prefetch_map(&map_v);
+    }
+    if (warp == 9) tc5::tmem_alloc<1>(tmem_slot, 512);
+    tc5::before_sync();
+    __syncthreads();
+    tc5::after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            int i = 0;
+            bool fine = true;
+            for (int t = t0; t < t1 && fine; ++t) {
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++i) {
+                    const int s = i % S::kStages;
+                    fine = fine && tc5::wait(&empty[s], ((i / S::kStages) & 1) ^ 1, given_up, &g_status);
+                    if (!fine) break;
+                    ofd::mbar_arrive_expect_tx(&full[s], S::kTileBytes);
+#pragma unroll
+                    for (int d = 0; d < S::kChunks; ++d)
+                        tc5::load_3d(ring + s * S::kTileBytes + d * 16384, kv ? &map_v : &map_k, d * 64, kh, k0 + base + t * kKeys, &full[s]);
+                }
+            }
+            if (!fine) ofd::mbar_drain_bounded(full, S::kStages, i, ofd::kDefaultWaitLimitNs);
+        }
+    } else if (warp == 9) {
+        const bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
+        const int steps_d = (a.head_dim + 15) / 16;
+        const uint32_t idesc_s = tc5::idesc_f16(128, kKeys, bf16, false), idesc_o = tc5::idesc_f16(128, steps_d * 16, bf16, true);
+        const uint32_t q_at = tc5::smem_u32(q_tiles), ring_at = tc5::smem_u32(ring);
+        int i = 0;  // tiles of the ring, in the order keys, values, keys, ...
+        int p_turn[2] = {0, 0};
+        bool fine = true;
+        for (int t = t0; t <= t1 && fine; ++t) {
+            const int sv = (i + S::kStages - 1) % S::kStages, sk = i % S::kStages;  // values of tile t - 1, keys of tile t
+            const int vi = i - 1, ki = i;
+            if (t > t0) {
+                fine = tc5::wait_warp(&full[sv], (vi / S::kStages) & 1, given_up, &g_status);
+                const int valid = nk - (base + (t - 1) * kKeys);
+                if (fine && valid < kKeys && (valid & 15)) {
+                    // rows behind the sequence's last key that the last step of 16 takes in: weights of zero, times what is there
+                    const int first = valid, count = 16 - (valid & 15);
+                    for (int n = lane; n < count * 8 * S::kChunks; n += 32) {
+                        const int d = n / (count * 8), rest_n = n % (count * 8);
+                        *reinterpret_cast<uint4 *>(ring + sv * S::kTileBytes + d * 16384 + (first + rest_n / 8) * 128 + (rest_n % 8) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    tc5::fence_async();
+                }
+                __syncwarp();
+            }
+            if (fine && t < t1) fine = tc5::wait_warp(&full[sk], (ki / S::kStages) & 1, given_up, &g_status);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (fine && t > t0 && t - 1 >= from[x] && t - 1 < to[x]) {
+                    fine = tc5::wait_warp(&p_ready[x], p_turn[x] & 1, given_up, &g_status);
+                    if (fine) {
+                        tc5::after_sync();
+                        if (lane == 0) {
+                            const int valid = min(nk - (base + (t - 1) * kKeys), kKeys), steps = (valid + 15) / 16;
+                            const uint32_t v_at = ring_at + sv * S::kTileBytes;
+                            for (int n = 0; n < steps; ++n)
+                                tc5::mma_f16_tmem(tmem + S::kOut + x * DP, tmem + x * kKeys + n * 8, tc5::desc_mn_major(v_at + n * 2048, 16384),
+                                                  idesc_o, p_turn[x] > 0 || n > 0);
+                            if (t == to[x]) tc5::commit(&o_full[x]);
+                        }
+                        ++p_turn[x];
+                    }
+                }
+                if (x == 1 && t > t0 && fine && lane == 0) tc5::commit(&empty[sv]);
+                if (fine && t < t1 && t >= from[x] && t < to[x]) {
+                    if (t == from[x]) {
+                        fine = tc5::wait_warp(&q_ready[x], 0, given_up, &g_status);
+                        tc5::after_sync();
+                    }
+                    if (fine && lane == 0) {
+                        const uint32_t k_at = ring_at + sk * S::kTileBytes;
+                        for (int n = 0; n < steps_d; ++n) {
+                            const uint32_t at = (n >> 2) * 16384 + (n & 3) * 32;
+                            tc5::mma_f16(tmem + x * kKeys, tc5::desc_k_major(q_at + x * S::kTileBytes + at), tc5::desc_k_major(k_at + at), idesc_s, n > 0);
+                        }
+                        tc5::commit(&s_full[x]);
+                    }
+                }
+            }
+            if (t < t1 && fine && lane == 0) tc5::commit(&empty[sk]);
+            i += 2;
+            __syncwarp();
+        }
+        if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
+            tc5::commit(&o_full[0]);
+            ofd::mbar_land(&o_full[0], 0, 0, ofd::kDefaultWaitLimitNs);
+        }
+    } else {
+        const int x = warp >> 2;
+        const int row = (warp & 3) * 32 + lane;  // of the half, and lane of tensor memory
+        const int r = r0 + x * kHalf + row, i = r / a.group, head = kh * a.group + r % a.group;
+        const bool there = r < rows;
+        const bool warp_there = r0 + x * kHalf + (warp & 3) * 32 < rows;
+        // ---- this half's queries into shared memory, pieces of 16 bytes; zeros where there are none
+        if (from[x] < to[x]) {
+            constexpr int kPieces = DP / 8;
+            for (int n = threadIdx.x & 127; n < kHalf * kPieces; n += 128) {
+                const int qr = n / kPieces, p = n % kPieces, rr = r0 + x * kHalf + qr;
+                uint4 val = make_uint4(0, 0, 0, 0);
+                if (rr < rows && p * 8 < a.head_dim)
+                    val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(q0 + rr / a.group) * a.q_stride_row +
+                                                           (kh * a.group + rr % a.group) * a.q_stride_head + p * 8);
+                *reinterpret_cast<uint4 *>(q_tiles + x * S::kTileBytes + (p >> 3) * 16384 + qr * 128 + (((p & 7) ^ (qr & 7)) << 4)) = val;
+            }
+            tc5::fence_async();
+            __syncwarp();
+            if (lane == 0) tc5::arrive(&q_ready[x]);
+        }
+        int my_lo = 0, my_hi = 0;
+        if (there) window(a, i, nq, nk, &my_lo, &my_hi);
+        float m = -INFINITY, l = 0.f;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + x * kKeys, o_at = tmem + lanes + S::kOut + x * DP;
+        bool fine = true;
+        int turn = 0;
+        for (int t = from[x]; t < to[x]; ++t, ++turn) {
+            fine = tc5::wait_warp(&s_full[x], turn & 1, given_up, &g_status);
+            if (!fine) break;
+            tc5::after_sync();
+            if (warp_there) {
+                uint32_t s[4][32];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) tc5::ld32(s[n], s_at + n * 32);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) tc5::ld_wait(s[n]);
+                const int j0 = base + t * kKeys, l0 = my_lo - j0, h0 = my_hi - j0;
+                if (__any_sync(0xffffffffu, l0 > 0 || h0 < kKeys)) {
+#pragma unroll
+                    for (int n = 0; n < kKeys; ++n)
+                        if (n < l0 || n >= h0) s[n >> 5][n & 31] = 0xff800000u;  // -infinity
+                }
+                float top[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    top[n] = __uint_as_float(s[n][0]);
+#pragma unroll
+                    for (int e = 1; e < 32; ++e) top[n] = fmaxf(top[n], __uint_as_float(s[n][e]));
+                }
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                float fade = 1.f;
+                if (most > m) {
+                    if (m == -INFINITY) {
+                        m = most;
+                    } else if ((most - m) * a.c > kLazy) {
+                        fade = ex2((m - most) * a.c);
+                        m = most;
+                    }
+                }
+                if (__any_sync(0xffffffffu, fade != 1.f)) {
+                    // the sums so far are all there: this tile's S came after the last tile's O
+                    l *= fade;
+#pragma unroll 1
+                    for (int n = 0; n < DP; n += 16) {
+                        uint32_t o[16];
+                        tc5::ld16(o, o_at + n);
+                        tc5::ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                        tc5::st16(o_at + n, o);
+                    }
+                }
+                const float shift = m == -INFINITY ? 0.f : -m * a.c;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float u = ex2(fmaf(__uint_as_float(s[n][e * 2]), a.c, shift));
+                        const float w = ex2(fmaf(__uint_as_float(s[n][e * 2 + 1]), a.c, shift));
+                        sum[e & 3] += u + w;
+                        p[e] = pack<T>(u, w);
+                    }
+                    tc5::st16(s_at + n * 16, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc5::st_wait();
+            }
+            tc5::before_sync();
+            __syncwarp();
+            if (lane == 0) tc5::arrive(&p_ready[x]);
+        }
+        // ---- out = O / l
+        const bool any = fine && from[x] < to[x];
+        if (any) {
+            fine = tc5::wait_warp(&o_full[x], 0, given_up, &g_status);
+            tc5::after_sync();
+        }
+        if (fine && warp_there) {
+            const int in_lo = max(my_lo, base + t0 * kKeys), in_hi = min(my_hi, base + t1 * kKeys);  // of this split
+            const bool sees = there && in_hi > in_lo;
+            const float back = sees ? 1.f / l : 0.f;
+            const long long at = (long long)(q0 + i) * a.q_heads + head;  // of [q_rows][q_heads]
+            T *const out = static_cast<T *>(a.out) + (long long)(q0 + i) * a.out_stride_row + head * a.out_stride_head;
+            float *const part = a.part + ((long long)split * a.q_rows * a.q_heads + at) * a.head_dim;
+            bool bad = false;
+#pragma unroll 1
+            for (int n = 0; n < DP; n += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                if (any) {
+                    tc5::ld32(o, o_at + n);
+                    tc5::ld_wait(o);
+                }
+                if (!there) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (n + e >= a.head_dim) break;
+                    float f[8];
+#pragma unroll
+                    for (int b = 0; b < 8; ++b) {
+                        f[b] = sees ? __uint_as_float(o[e + b]) * back : 0.f;
+                        bad |= !(fabsf(f[b]) < INFINITY);
+                    }
+                    if (a.splits == 1) {
+                        *reinterpret_cast<uint4 *>(out + n + e) = make_uint4(pack<T>(f[0], f[1]), pack<T>(f[2], f[3]), pack<T>(f[4], f[5]), pack<T>(f[6], f[7]));
+                    } else {
+                        *reinterpret_cast<float4 *>(part + n + e) = make_float4(f[0], f[1], f[2], f[3]);
+                        *reinterpret_cast<float4 *>(part + n + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
+                    }
+                }
+            }
+            float lse = sees ? m * a.c + log2f(l) : -INFINITY;
+            __syncwarp();
+            for (uint32_t again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
+                const int who = __ffs(again) - 1;
+                const int rr = r0 + x * kHalf + (warp & 3) * 32 + who, ii = rr / a.group, hh = kh * a.group + rr % a.group;
+                const int klo = __shfl_sync(0xffffffffu, in_lo, who), khi = __shfl_sync(0xffffffffu, in_hi, who);
+                const long long aa = (long long)(q0 + ii) * a.q_heads + hh;
+                const float2 ml = redo_row<T>(static_cast<const T *>(a.q) + (long long)(q0 + ii) * a.q_stride_row + hh * a.q_stride_head,
+                                              static_cast<const T *>(a.k) + (long long)k0 * a.k_stride_row + kh * a.k_stride_head,
+                                              static_cast<const T *>(a.v) + (long long)k0 * a.v_stride_row + kh * a.v_stride_head, a.k_stride_row,
+                                              a.v_stride_row, a.head_dim, a.c, klo, khi,
+                                              a.part + ((long long)split * a.q_rows * a.q_heads + aa) * a.head_dim,
+                                              a.splits > 1 ? nullptr : static_cast<T *>(a.out) + (long long)(q0 + ii) * a.out_stride_row + hh * a.out_stride_head);
+                if (lane == who) lse = ml.x * a.c + log2f(ml.y);
+            }
+            if (a.splits > 1 && there) a.part_lse[(long long)split * a.q_rows * a.q_heads + at] = lse;
+        }
+    }
+    __syncwarp();
+    tc5::before_sync();
+    __syncthreads();
+    tc5::after_sync();
+    if (warp == 9) tc5::tmem_free<1>(tmem, 512);
+}
+
+// The splits' results joined: out = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A warp to a query and head.
+template <class T>
+__global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
+    const int lane = threadIdx.x & 31;
+    const long long per = (long long)a.max_q * a.q_heads;
+    const long long all = per * a.sequences;
+    for (long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); w < all; w += (long long)gridDim.x * 4) {
+        const int seq = (int)(w / per), i = (int)(w % per / a.q_heads), head = (int)(w % a.q_heads);
+        int q0, nq, k0, nk, lo, hi;
+        span(a.q_start, a.q_used, seq, a.q_rows, a.max_q, &q0, &nq);
+        if (i >= nq) continue;
+        span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
+        window(a, i, nq, nk, &lo, &hi);
+        const long long at = (long long)(q0 + i) * a.q_heads + head, step = (long long)a.q_rows * a.q_heads;
+        float top = -INFINITY;
+        for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_lse[z * step + at]);
+        const float from = top == -INFINITY ? 0.f : top;
+        float total = 0.f, acc[4] = {};
+        for (int z = 0; z < a.splits; ++z) {
+            const float lse = a.part_lse[z * step + at];
+            if (lse == -INFINITY) continue;  // nothing seen there (or nothing but -infinity)
+            const float f = ex2(lse - from);
+            total += f;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (lane + 32 * n < a.head_dim) acc[n] = fmaf(f, a.part[(z * step + at) * a.head_dim + lane + 32 * n], acc[n]);
+        }
+        T *const out = static_cast<T *>(a.out) + (long long)(q0 + i) * a.out_stride_row + head * a.out_stride_head;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (lane + 32 * n < a.head_dim) out[lane + 32 * n] = ofe::from_float<T>(hi > lo ? acc[n] / total : 0.f);
+    }
+}
+
+// Into how many pieces a tile's keys go: enough blocks to fill the SMs, two tiles of keys to a piece at least.
+int splits_for(const openfish_b200_attention_t *a, int sms) {
+    const long long group = a->q_heads / a->kv_heads;
+    const long long blocks = (a->max_q * group + 2 * kHalf - 1) / (2 * kHalf) * a->kv_heads * a->sequences;
+    long long keys = a->max_k;
+    if (a->window_left >= 0 && a->window_right >= 0) {
+        const long long seen = (long long)a->window_left + a->window_right + 1 + 2 * kHalf / group;
+        if (seen < keys) keys = seen;
+    }
+    const long long tiles = (keys + kKeys - 1) / kKeys;
+    long long n = sms / blocks;
+    if (n > tiles / 2) n = tiles / 2;
+    if (n > 64) n = 64;
+    return n < 1 ? 1 : (int)n;
+}
+
+bool heads_map(CUtensorMap *map, bool bf16, const void *base, const openfish_b200_attention_t *a, long long stride_row, long long stride_head) {
+    const cuuint64_t dims[3] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->kv_heads, (cuuint64_t)a->k_rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)(a->kv_heads > 1 ? stride_head : 128) * 2, (cuuint64_t)(a->k_rows > 1 ? stride_row : 128) * 2};
+    const cuuint32_t box[3] = {64, 1, kKeys};
+    return tc5::make_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box);
+}
+
+template <class T, int DP>
+int launch(const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
+    const auto kernel = attention_kernel<T, DP>;
+    if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kBytes))) return rc;
+    const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
+    kernel<<<(unsigned)blocks, kThreads, Shape<DP>::kBytes, stream>>>(a, mk, mv);
+    if (const int rc = ofe::launched()) return rc;
+    if (a.splits == 1) return OPENFISH_B200_OK;
+    const long long joins = ((long long)a.max_q * a.q_heads * a.sequences + 3) / 4;
+    attention_join_kernel<T><<<(unsigned)(joins < 16384 ? joins : 16384), 128, 0, stream>>>(a);
+    return ofe::launched();
+}
+
+size_t part_bytes(const openfish_b200_attention_t *a, int splits) {
+    return splits == 1 ? 0 : (size_t)splits * a->q_rows * a->q_heads * (a->head_dim + 1) * sizeof(float);
+}
 
 }  // namespace
 
-extern "C" size_t ofb_attention_workspace(const openfish_b200_attention_t *) { return 0; }
+extern "C" size_t ofb_attention_workspace(const openfish_b200_attention_t *a) {
+    int sms = 0;
+    if (ofe::sm_count(&sms)) return 0;
+    return part_bytes(a, splits_for(a, sms));
+}
 
-extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *a) {
-    const dim3 grid((unsigned)(((long long)a->max_q * a->q_heads + 3) / 4), a->sequences < 65535 ? a->sequences : 65535);
-    if (a->dtype == OPENFISH_B200_F16) attention_simple_kernel<__half><<<grid, 128, 0, (cudaStream_t)stream>>>(*a);
-    else attention_simple_kernel<__nv_bfloat16><<<grid, 128, 0, (cudaStream_t)stream>>>(*a);
-    return ofe::launched();
+extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
+    int sms = 0;
+    if (const int rc = ofe::sm_count(&sms)) return rc;
+    Args a;
+    a.q_start = p->q_start; a.k_start = p->k_start; a.q_used = p->q_used; a.k_used = p->k_used;
+    a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out;
+    // a stride counts only where there is a second element along it
+    a.q_stride_row = p->q_stride_row; a.q_stride_head = p->q_heads > 1 ? p->q_stride_head : 0;
+    a.k_stride_row = p->k_stride_row; a.k_stride_head = p->kv_heads > 1 ? p->k_stride_head : 0;
+    a.v_stride_row = p->v_stride_row; a.v_stride_head = p->kv_heads > 1 ? p->v_stride_head : 0;
+    a.out_stride_row = p->out_stride_row; a.out_stride_head = p->q_heads > 1 ? p->out_stride_head : 0;
+    a.q_rows = (int)p->q_rows; a.k_rows = (int)p->k_rows; a.q_heads = p->q_heads; a.kv_heads = p->kv_heads; a.group = p->q_heads / p->kv_heads;
+    a.head_dim = p->head_dim; a.sequences = p->sequences; a.max_q = p->max_q; a.max_k = p->max_k;
+    const int wide = 1 << 30;  // beyond any sequence
+    a.left = p->window_left < wide ? p->window_left : -1;
+    a.right = p->window_right < wide ? p->window_right : -1;
+    a.c = p->scale * 1.4426950408889634f;
+    a.tiles = (int)(((long long)p->max_q * a.group + 2 * kHalf - 1) / (2 * kHalf));
+    a.splits = splits_for(p, sms);
+    a.part_lse = static_cast<float *>(p->workspace);
+    a.part = a.part_lse;
+    if (a.splits > 1) {
+        // sums first: their rows are read and written 16 bytes at a time
+        a.part = static_cast<float *>(p->workspace);
+        a.part_lse = a.part + (size_t)a.splits * a.q_rows * a.q_heads * a.head_dim;
+    }
+    const bool bf16 = p->dtype == OPENFISH_B200_BF16;
+    CUtensorMap mk, mv;
+    openfish_b200_attention_t none = *p;  // no keys at all: the kernel copies nothing, but a map has to be one of something
+    const void *k = p->k, *v = p->v;
+    if (p->k_rows == 0) {
+        none.k_rows = none.kv_heads = 1;
+        k = v = p->q;
+    }
+    if (!heads_map(&mk, bf16, k, &none, p->k_stride_row, p->k_stride_head) || !heads_map(&mv, bf16, v, &none, p->v_stride_row, p->v_stride_head))
+        return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
+    if (p->head_dim <= 64) return bf16 ? launch<__nv_bfloat16, 64>(a, mk, mv, (cudaStream_t)stream) : launch<__half, 64>(a, mk, mv, (cudaStream_t)stream);
+    return bf16 ? launch<__nv_bfloat16, 128>(a, mk, mv, (cudaStream_t)stream) : launch<__half, 128>(a, mk, mv, (cudaStream_t)stream);
 }
 
 extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }

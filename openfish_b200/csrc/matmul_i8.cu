@@ -160,8 +160,7 @@ __global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const
             walk.at(t, &tm, &tn);
             const int m0 = tm * 128 * CG + rank * 128 + quarter * 32, n0 = tn * BN;
             const float xs = m0 + lane < a.rows ? a.x_scale[m0 + lane] : 0.f;
-            const bool fine = tc5::wait(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status);
-            if (__any_sync(0xffffffffu, !fine)) break;
+            if (!tc5::wait_warp(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status)) break;
             tc5::after_sync();
 #pragma unroll 1
             for (int c = 0; c < BN; c += 64, ++turn) {
