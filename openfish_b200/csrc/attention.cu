@@ -10,10 +10,12 @@
 //
 //   warps 0-3, 4-7   the softmax of the first and second half, a thread to a row
 //   warp 8           asynchronous copies of the keys' and values' tiles into a ring in shared memory
-//   warp 9           matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there
+//   warps 9, 10      a half's matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there
 //
-// P takes the place of the S it came from.  While one half's weights are worked out, the matrix unit is busy with the other
-// half's: O += P V of the last tile, then S of the next one.
+// Heads of up to 64 have room for P beside S in tensor memory: the next tile's S is formed while this tile's weights are
+// worked out.  With larger heads P takes the place of its S, and a half's products follow one another: the first 64
+// keys' O += P V while the others' weights are still worked out, the rest, S of the next tile.  The matrix unit has the other
+// half's products in the meantime.
 #include <math.h>
 #include <stdint.h>
 
@@ -26,7 +28,7 @@ __device__ int g_status;  // of the kernels on this device: a wait that ran out
 
 constexpr int kHalf = 128;  // rows of a half
 constexpr int kKeys = 128;  // keys of a tile
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled: weights up to 256
 
 struct Args {
@@ -36,6 +38,7 @@ struct Args {
     float *part, *part_lse;  // of a split: [split][q_rows][q_heads][head_dim] and [split][q_rows][q_heads]
     long long q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head, out_stride_row, out_stride_head;
     int q_rows, k_rows, q_heads, kv_heads, group, head_dim, sequences, max_q, max_k, left, right;
+    uint32_t group_mul, group_shift;  // r / group = (mulhi(r, group_mul) + r) >> group_shift for r < 2^30
     int tiles, splits;  // of 256 rows of the longest sequence; pieces of a tile's keys
     float c;
 };
@@ -55,9 +58,31 @@ __device__ __forceinline__ void window(const Args &a, int i, int nq, int nk, int
     *hi = a.right < 0 ? nk : min(place + a.right + 1, nk);
 }
 
+__device__ __forceinline__ int by_group(const Args &a, int r) { return (int)((__umulhi((uint32_t)r, a.group_mul) + (uint32_t)r) >> a.group_shift); }
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The largest of three numbers (a NaN is passed over).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// Two fp32 operations in an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 y;
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%6, %7};\n\t"
+        "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 y;
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return y;
 }
 template <class T>
@@ -78,8 +103,10 @@ struct Shape {
     static constexpr int kChunks = DP / 64;                   // of 64 elements, 128 bytes
     static constexpr int kTileBytes = kChunks * 128 * 128;    // 128 rows
     static constexpr int kStages = DP == 64 ? 10 : 5;
-    static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes + (2 * kStages + 8) * 8 + 16;
-    static constexpr int kOut = 256;                          // the sums' first column of tensor memory, behind two S
+    static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes + (2 * kStages + 12) * 8 + 16;
+    // columns of tensor memory: two S, two O, and two P where there is room
+    static constexpr bool kApart = DP == 64;
+    static constexpr int kOut = 2 * kKeys, kWeights = kApart ? kOut + 2 * DP : 0, kWeightsStep = kApart ? kKeys / 2 : kKeys;
 };
 
 // One row again, by a warp, straight from its definition and reading only the keys that the row sees.  A matrix
@@ -144,8 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
         lo[x] = hi[x] = 0;
         if (first < rows) {
             int unused;
-            window(a, first / a.group, nq, nk, &lo[x], &unused);
-            window(a, last / a.group, nq, nk, &unused, &hi[x]);
+            window(a, by_group(a, first), nq, nk, &lo[x], &unused);
+            window(a, by_group(a, last), nq, nk, &unused, &hi[x]);
             if (hi[x] <= lo[x]) lo[x] = hi[x] = 0;
         }
     }
@@ -167,21 +194,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
     uint8_t *const q_tiles = raw + ((1024 - (tc5::smem_u32(raw) & 1023)) & 1023);
     uint8_t *const ring = q_tiles + 2 * S::kTileBytes;
     uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kTileBytes), *const empty = full + S::kStages;
-    uint64_t *const q_ready = empty + S::kStages, *const s_full = q_ready + 2, *const p_ready = s_full + 2, *const o_full = p_ready + 2;
-    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+    uint64_t *const q_ready = empty + S::kStages, *const s_full = q_ready + 2, *const s_read = s_full + 2, *const p_first = s_read + 2;
+    uint64_t *const p_ready = p_first + 2, *const o_done = p_ready + 2;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_done + 2);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     if (threadIdx.x == 0) {
         *given_up = 0;
         for (int i = 0; i < S::kStages; ++i) {
             ofd::mbar_init(&full[i], 1);
-            ofd::mbar_init(&empty[i], 1);
+            ofd::mbar_init(&empty[i], 2);
         }
         for (int x = 0; x < 2; ++x) {
             ofd::mbar_init(&q_ready[x], 4);
             ofd::mbar_init(&s_full[x], 1);
+            ofd::mbar_init(&s_read[x], 4);
+            ofd::mbar_init(&p_first[x], 4);
             ofd::mbar_init(&p_ready[x], 4);
-            ofd::mbar_init(&o_full[x], 1);
+            ofd::mbar_init(&o_done[x], 1);
         }
         ofd::mbar_fence_init();
         tc5::prefetch_map(&map_k);
@@ -195,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
 
     if (warp == 8) {
         if (lane == 0) {
-            int i = 0;
+            int i = 0;  // tiles of the ring, in the order keys, values, keys, ...
             bool fine = true;
             for (int t = t0; t < t1 && fine; ++t) {
 #pragma unroll
@@ -211,165 +241,235 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
             }
             if (!fine) ofd::mbar_drain_bounded(full, S::kStages, i, ofd::kDefaultWaitLimitNs);
         }
-    } else if (warp == 9) {
-        const bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
-        const int steps_d = (a.head_dim + 15) / 16;
-        const uint32_t idesc_s = tc5::idesc_f16(128, kKeys, bf16, false), idesc_o = tc5::idesc_f16(128, steps_d * 16, bf16, true);
-        const uint32_t q_at = tc5::smem_u32(q_tiles), ring_at = tc5::smem_u32(ring);
-        int i = 0;  // tiles of the ring, in the order keys, values, keys, ...
-        int p_turn[2] = {0, 0};
+    } else if (warp >= 9) {
+        // The instructions are issued one after the other by one thread, whose own pace counts: descriptors are sums with
+        // constants, loops are unrolled.
+        const int x = warp - 9;
+        constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+        constexpr uint32_t idesc_s = tc5::idesc_f16(128, kKeys, bf16, false), idesc_o = tc5::idesc_f16(128, DP, bf16, true);
+        const uint64_t q_desc = tc5::desc_k_major(tc5::smem_u32(q_tiles) + x * S::kTileBytes), k_desc = tc5::desc_k_major(tc5::smem_u32(ring));
+        const uint64_t v_desc = tc5::desc_mn_major(tc5::smem_u32(ring), 16384);
+        const uint32_t s_at = tmem + x * kKeys, o_at = tmem + S::kOut + x * DP, p_at = tmem + S::kWeights + x * S::kWeightsStep;
+        int sk = 0, sv = 0;               // the ring's places of tile t's keys and of tile t - 1's values
+        uint32_t k_turn = 0, v_turn = 0;  // and their turns
+        uint32_t turn = 0;                // tiles of this half whose values have been taken
         bool fine = true;
-        for (int t = t0; t <= t1 && fine; ++t) {
-            const int sv = (i + S::kStages - 1) % S::kStages, sk = i % S::kStages;  // values of tile t - 1, keys of tile t
-            const int vi = i - 1, ki = i;
-            if (t > t0) {
-                fine = tc5::wait_warp(&full[sv], (vi / S::kStages) & 1, given_up, &g_status);
-                const int valid = nk - (base + (t - 1) * kKeys);
-                if (fine && valid < kKeys && (valid & 15)) {
-                    // rows behind the sequence's last key that the last step of 16 takes in: weights of zero, times what is there
-                    const int first = valid, count = 16 - (valid & 15);
+        const auto scores = [&](int t) {  // S = Q K^T of tile t; true if there is none
+            fine = fine && tc5::wait_warp(&full[sk], k_turn, given_up, &g_status);
+            if (fine && t >= from[x] && t < to[x]) {
+                if (t == from[x]) fine = tc5::wait_warp(&q_ready[x], 0, given_up, &g_status);
+                else if (S::kApart) fine = tc5::wait_warp(&s_read[x], (t - from[x] - 1) & 1, given_up, &g_status);
+                tc5::after_sync();
+                const uint64_t kd = k_desc + (uint32_t)(sk * (S::kTileBytes >> 4));
+                if (fine && tc5::elect()) {
+#pragma unroll
+                    for (int n = 0; n < DP / 16; ++n) {
+                        const uint32_t at = ((n >> 2) * 16384 + (n & 3) * 32) >> 4;
+                        tc5::mma_f16(s_at, q_desc + at, kd + at, idesc_s, n > 0);
+                    }
+                    tc5::commit(&s_full[x]);
+                }
+            }
+            if (fine && tc5::elect()) tc5::commit(&empty[sk]);
+        };
+        const auto sums = [&](int t) {  // O += P V of tile t
+            fine = fine && tc5::wait_warp(&full[sv], v_turn, given_up, &g_status);
+            if (fine && t >= from[x] && t < to[x]) {
+                const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
+                if (valid & 15) {
+                    // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
+                    const int count = 16 - (valid & 15);
                     for (int n = lane; n < count * 8 * S::kChunks; n += 32) {
-                        const int d = n / (count * 8), rest_n = n % (count * 8);
-                        *reinterpret_cast<uint4 *>(ring + sv * S::kTileBytes + d * 16384 + (first + rest_n / 8) * 128 + (rest_n % 8) * 16) =
-                            make_uint4(0, 0, 0, 0);
+                        const int d = n / (count * 8), in = n % (count * 8);
+                        *reinterpret_cast<uint4 *>(ring + sv * S::kTileBytes + d * 16384 + valid * 128 + in * 16) = make_uint4(0, 0, 0, 0);
                     }
                     tc5::fence_async();
+                    __syncwarp();
                 }
-                __syncwarp();
-            }
-            if (fine && t < t1) fine = tc5::wait_warp(&full[sk], (ki / S::kStages) & 1, given_up, &g_status);
+                const uint64_t vd = v_desc + (uint32_t)(sv * (S::kTileBytes >> 4));
+                fine = tc5::wait_warp(&p_first[x], turn & 1, given_up, &g_status);
+                tc5::after_sync();
+                if (fine && tc5::elect()) {
+                    if (steps >= 4) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if (fine && t > t0 && t - 1 >= from[x] && t - 1 < to[x]) {
-                    fine = tc5::wait_warp(&p_ready[x], p_turn[x] & 1, given_up, &g_status);
-                    if (fine) {
-                        tc5::after_sync();
-                        if (lane == 0) {
-                            const int valid = min(nk - (base + (t - 1) * kKeys), kKeys), steps = (valid + 15) / 16;
-                            const uint32_t v_at = ring_at + sv * S::kTileBytes;
-                            for (int n = 0; n < steps; ++n)
-                                tc5::mma_f16_tmem(tmem + S::kOut + x * DP, tmem + x * kKeys + n * 8, tc5::desc_mn_major(v_at + n * 2048, 16384),
-                                                  idesc_o, p_turn[x] > 0 || n > 0);
-                            if (t == to[x]) tc5::commit(&o_full[x]);
-                        }
-                        ++p_turn[x];
+                        for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, turn > 0 || n > 0);
+                    } else {
+                        for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, turn > 0 || n > 0);
                     }
                 }
-                if (x == 1 && t > t0 && fine && lane == 0) tc5::commit(&empty[sv]);
-                if (fine && t < t1 && t >= from[x] && t < to[x]) {
-                    if (t == from[x]) {
-                        fine = tc5::wait_warp(&q_ready[x], 0, given_up, &g_status);
-                        tc5::after_sync();
+                fine = fine && tc5::wait_warp(&p_ready[x], turn & 1, given_up, &g_status);
+                tc5::after_sync();
+                if (fine && tc5::elect()) {
+                    if (steps == 8) {
+#pragma unroll
+                        for (int n = 4; n < 8; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, true);
+                    } else {
+                        for (int n = 4; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, true);
                     }
-                    if (fine && lane == 0) {
-                        const uint32_t k_at = ring_at + sk * S::kTileBytes;
-                        for (int n = 0; n < steps_d; ++n) {
-                            const uint32_t at = (n >> 2) * 16384 + (n & 3) * 32;
-                            tc5::mma_f16(tmem + x * kKeys, tc5::desc_k_major(q_at + x * S::kTileBytes + at), tc5::desc_k_major(k_at + at), idesc_s, n > 0);
-                        }
-                        tc5::commit(&s_full[x]);
-                    }
+                    if (S::kApart || t + 1 == to[x]) tc5::commit(&o_done[x]);
                 }
+                ++turn;
             }
-            if (t < t1 && fine && lane == 0) tc5::commit(&empty[sk]);
-            i += 2;
+            if (fine && tc5::elect()) tc5::commit(&empty[sv]);
+        };
+        for (int t = t0; t <= t1 && fine; ++t) {
+            if (S::kApart && t < t1) scores(t);
+            if (t > t0) sums(t - 1);
+            if (!S::kApart && t < t1) scores(t);
+            // keys and values take turns in the ring
+            sv = sk + 1;
+            v_turn = k_turn;
+            if (sv == S::kStages) sv = 0, v_turn ^= 1;
+            sk = sv + 1;
+            k_turn = v_turn;
+            if (sk == S::kStages) sk = 0, k_turn ^= 1;
             __syncwarp();
         }
         if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
-            tc5::commit(&o_full[0]);
-            ofd::mbar_land(&o_full[0], 0, 0, ofd::kDefaultWaitLimitNs);
+            tc5::commit(&o_done[x]);
+            ofd::mbar_land(&o_done[x], 0, 0, ofd::kDefaultWaitLimitNs);
         }
     } else {
         const int x = warp >> 2;
         const int row = (warp & 3) * 32 + lane;  // of the half, and lane of tensor memory
-        const int r = r0 + x * kHalf + row, i = r / a.group, head = kh * a.group + r % a.group;
+        const int r = r0 + x * kHalf + row, i = by_group(a, r), head = kh * a.group + r - i * a.group;
         const bool there = r < rows;
         const bool warp_there = r0 + x * kHalf + (warp & 3) * 32 < rows;
         // ---- this half's queries into shared memory, pieces of 16 bytes; zeros where there are none
         if (from[x] < to[x]) {
             constexpr int kPieces = DP / 8;
+#pragma unroll 4
             for (int n = threadIdx.x & 127; n < kHalf * kPieces; n += 128) {
-                const int qr = n / kPieces, p = n % kPieces, rr = r0 + x * kHalf + qr;
+                const int qr = n / kPieces, p = n % kPieces, rr = r0 + x * kHalf + qr, ri = by_group(a, rr);
                 uint4 val = make_uint4(0, 0, 0, 0);
                 if (rr < rows && p * 8 < a.head_dim)
-                    val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(q0 + rr / a.group) * a.q_stride_row +
-                                                           (kh * a.group + rr % a.group) * a.q_stride_head + p * 8);
+                    val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(q0 + ri) * a.q_stride_row +
+                                                           (kh * a.group + rr - ri * a.group) * a.q_stride_head + p * 8);
                 *reinterpret_cast<uint4 *>(q_tiles + x * S::kTileBytes + (p >> 3) * 16384 + qr * 128 + (((p & 7) ^ (qr & 7)) << 4)) = val;
             }
             tc5::fence_async();
             __syncwarp();
             if (lane == 0) tc5::arrive(&q_ready[x]);
         }
-        int my_lo = 0, my_hi = 0;
-        if (there) window(a, i, nq, nk, &my_lo, &my_hi);
+        // ---- the keys this row sees, and between them the first and the last row of the warp (rows that are not there
+        // are given the last row's)
+        int my_lo, my_hi;
+        window(a, by_group(a, min(r, rows - 1)), nq, nk, &my_lo, &my_hi);
+        const int first_lo = __shfl_sync(0xffffffffu, my_lo, 0), first_hi = __shfl_sync(0xffffffffu, my_hi, 0);
+        const int last_lo = __shfl_sync(0xffffffffu, my_lo, 31), last_hi = __shfl_sync(0xffffffffu, my_hi, 31);
         float m = -INFINITY, l = 0.f;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + x * kKeys, o_at = tmem + lanes + S::kOut + x * DP;
+        const uint32_t p_at = tmem + lanes + S::kWeights + x * S::kWeightsStep;
         bool fine = true;
         int turn = 0;
         for (int t = from[x]; t < to[x]; ++t, ++turn) {
             fine = tc5::wait_warp(&s_full[x], turn & 1, given_up, &g_status);
             if (!fine) break;
             tc5::after_sync();
-            if (warp_there) {
-                uint32_t s[4][32];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) tc5::ld32(s[n], s_at + n * 32);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) tc5::ld_wait(s[n]);
-                const int j0 = base + t * kKeys, l0 = my_lo - j0, h0 = my_hi - j0;
-                if (__any_sync(0xffffffffu, l0 > 0 || h0 < kKeys)) {
-#pragma unroll
-                    for (int n = 0; n < kKeys; ++n)
-                        if (n < l0 || n >= h0) s[n >> 5][n & 31] = 0xff800000u;  // -infinity
+            if (!warp_there) {  // nothing but rows that are not there: their weights are whatever lies in the place
+                __syncwarp();
+                if (S::kApart && lane == 0) tc5::arrive(&s_read[x]);
+                // (not before the other warps' weights of the last tile have been taken: an arrival counts for the turn it finds)
+                if (S::kApart && turn > 0) fine = tc5::wait_warp(&o_done[x], (turn - 1) & 1, given_up, &g_status);
+                if (!fine) break;
+                if (lane == 0) {
+                    tc5::arrive(&p_first[x]);
+                    tc5::arrive(&p_ready[x]);
                 }
-                float top[4];
+                continue;
+            }
+            uint32_t s[4][32];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    top[n] = __uint_as_float(s[n][0]);
+            for (int n = 0; n < 4; ++n) tc5::ld32(s[n], s_at + n * 32);
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) top[n] = fmaxf(top[n], __uint_as_float(s[n][e]));
+            for (int n = 0; n < 4; ++n) tc5::ld_wait(s[n]);
+            if (S::kApart) {
+                tc5::before_sync();
+                __syncwarp();
+                if (lane == 0) tc5::arrive(&s_read[x]);
+            }
+            // 32 keys at a time: seen by every row, by none, or by some
+            const int j0 = base + t * kKeys;
+            bool none[4];
+            float most = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int b = j0 + n * 32, e = b + 32;
+                none[n] = first_lo >= e || last_hi <= b;
+                if (none[n]) continue;
+                if (last_lo > b || first_hi < e) {
+                    const int lo_n = max(my_lo - b, 0), hi_n = min(my_hi - b, 32);
+                    const uint32_t keep = hi_n <= lo_n ? 0u : (0xffffffffu >> (32 - (hi_n - lo_n))) << lo_n;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (!(keep >> c & 1)) s[n][c] = 0xff800000u;  // -infinity
                 }
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                float fade = 1.f;
-                if (most > m) {
-                    if (m == -INFINITY) {
-                        m = most;
-                    } else if ((most - m) * a.c > kLazy) {
-                        fade = ex2((m - most) * a.c);
-                        m = most;
-                    }
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    top[0] = max3(top[0], __uint_as_float(s[n][c]), __uint_as_float(s[n][c + 1]));
+                    top[1] = max3(top[1], __uint_as_float(s[n][c + 2]), __uint_as_float(s[n][c + 3]));
                 }
-                if (__any_sync(0xffffffffu, fade != 1.f)) {
-                    // the sums so far are all there: this tile's S came after the last tile's O
-                    l *= fade;
+                most = max3(most, top[0], top[1]);
+            }
+            float fade = 1.f;
+            if (most > m) {
+                if (m == -INFINITY) {
+                    m = most;
+                } else if ((most - m) * a.c > kLazy) {
+                    fade = ex2((m - most) * a.c);
+                    m = most;
+                }
+            }
+            if (S::kApart && turn > 0) {  // the last tile's weights have been taken, and its sums are there
+                fine = tc5::wait_warp(&o_done[x], (turn - 1) & 1, given_up, &g_status);
+                if (!fine) break;
+                tc5::after_sync();
+            }
+            if (__any_sync(0xffffffffu, fade != 1.f)) {
+                // the sums so far are all there: where P has S's place, this tile's S came after the last tile's O
+                l *= fade;
 #pragma unroll 1
-                    for (int n = 0; n < DP; n += 16) {
-                        uint32_t o[16];
-                        tc5::ld16(o, o_at + n);
-                        tc5::ld_wait(o);
+                for (int n = 0; n < DP; n += 16) {
+                    uint32_t o[16];
+                    tc5::ld16(o, o_at + n);
+                    tc5::ld_wait(o);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                        tc5::st16(o_at + n, o);
-                    }
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                    tc5::st16(o_at + n, o);
                 }
-                const float shift = m == -INFINITY ? 0.f : -m * a.c;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            }
+            const float shift = m == -INFINITY ? 0.f : -m * a.c;
+            const float2 c2 = {a.c, a.c}, shift2 = {shift, shift};
+            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    uint32_t p[16];
+            for (int n = 0; n < 4; ++n) {
+                uint32_t p[16];
+                if (none[n]) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) p[e] = 0;
+                } else {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float u = ex2(fmaf(__uint_as_float(s[n][e * 2]), a.c, shift));
-                        const float w = ex2(fmaf(__uint_as_float(s[n][e * 2 + 1]), a.c, shift));
-                        sum[e & 3] += u + w;
-                        p[e] = pack<T>(u, w);
+                        float2 z = fma2({__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1])}, c2, shift2);
+                        z.x = ex2(z.x);
+                        z.y = ex2(z.y);
+                        sum[e & 1] = add2(sum[e & 1], z);
+                        p[e] = pack<T>(z.x, z.y);
                     }
-                    tc5::st16(s_at + n * 16, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc5::st_wait();
+                tc5::st16(p_at + n * 16, p);
+                if (n == 1) {
+                    tc5::st_wait();
+                    tc5::before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc5::arrive(&p_first[x]);
+                }
             }
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+            tc5::st_wait();
             tc5::before_sync();
             __syncwarp();
             if (lane == 0) tc5::arrive(&p_ready[x]);
@@ -377,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
         // ---- out = O / l
         const bool any = fine && from[x] < to[x];
         if (any) {
-            fine = tc5::wait_warp(&o_full[x], 0, given_up, &g_status);
+            fine = tc5::wait_warp(&o_done[x], S::kApart ? (turn - 1) & 1 : 0, given_up, &g_status);
             tc5::after_sync();
         }
         if (fine && warp_there) {
@@ -418,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
             __syncwarp();
             for (uint32_t again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
                 const int who = __ffs(again) - 1;
-                const int rr = r0 + x * kHalf + (warp & 3) * 32 + who, ii = rr / a.group, hh = kh * a.group + rr % a.group;
+                const int rr = r0 + x * kHalf + (warp & 3) * 32 + who, ii = by_group(a, rr), hh = kh * a.group + rr - ii * a.group;
                 const int klo = __shfl_sync(0xffffffffu, in_lo, who), khi = __shfl_sync(0xffffffffu, in_hi, who);
                 const long long aa = (long long)(q0 + ii) * a.q_heads + hh;
                 const float2 ml = redo_row<T>(static_cast<const T *>(a.q) + (long long)(q0 + ii) * a.q_stride_row + hh * a.q_stride_head,
@@ -537,6 +637,10 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     const int wide = 1 << 30;  // beyond any sequence
     a.left = p->window_left < wide ? p->window_left : -1;
     a.right = p->window_right < wide ? p->window_right : -1;
+    int bits = 0;
+    while ((1LL << bits) < a.group) ++bits;
+    a.group_shift = (uint32_t)bits;
+    a.group_mul = (uint32_t)(((1ull << 32) * ((1ull << bits) - (unsigned)a.group)) / (unsigned)a.group + 1);
     a.c = p->scale * 1.4426950408889634f;
     a.tiles = (int)(((long long)p->max_q * a.group + 2 * kHalf - 1) / (2 * kHalf));
     a.splits = splits_for(p, sms);
