@@ -103,7 +103,7 @@ struct Shape {
     static constexpr int kChunks = DP / 64;                   // of 64 elements, 128 bytes
     static constexpr int kTileBytes = kChunks * 128 * 128;    // 128 rows
     static constexpr int kStages = DP == 64 ? 10 : 5;
-    static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes + (2 * kStages + 12) * 8 + 16;
+    static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes + (2 * kStages + 14) * 8 + 16;
     // columns of tensor memory: two S, two O, and two P where there is room
     static constexpr bool kApart = DP == 64;
     static constexpr int kOut = 2 * kKeys, kWeights = kApart ? kOut + 2 * DP : 0, kWeightsStep = kApart ? kKeys / 2 : kKeys;
@@ -195,8 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
     uint8_t *const ring = q_tiles + 2 * S::kTileBytes;
     uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kTileBytes), *const empty = full + S::kStages;
     uint64_t *const q_ready = empty + S::kStages, *const s_full = q_ready + 2, *const s_read = s_full + 2, *const p_first = s_read + 2;
-    uint64_t *const p_ready = p_first + 2, *const o_done = p_ready + 2;
-    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_done + 2);
+    uint64_t *const p_ready = p_first + 2, *const o_done = p_ready + 2, *const my_turn = o_done + 2;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(my_turn + 2);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     if (threadIdx.x == 0) {
@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
             ofd::mbar_init(&p_first[x], 4);
             ofd::mbar_init(&p_ready[x], 4);
             ofd::mbar_init(&o_done[x], 1);
+            ofd::mbar_init(&my_turn[x], 1);
         }
         ofd::mbar_fence_init();
         tc5::prefetch_map(&map_k);
@@ -298,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
                     }
                 }
                 fine = fine && tc5::wait_warp(&p_ready[x], turn & 1, given_up, &g_status);
+                if (!S::kApart) fine = fine && tc5::wait_warp(&my_turn[x], (t + 1 - t0 + x + 1) & 1, given_up, &g_status);
                 tc5::after_sync();
                 if (fine && tc5::elect()) {
                     if (steps == 8) {
@@ -315,7 +317,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
         for (int t = t0; t <= t1 && fine; ++t) {
             if (S::kApart && t < t1) scores(t);
             if (t > t0) sums(t - 1);
-            if (!S::kApart && t < t1) scores(t);
+            if (!S::kApart) {
+                // The halves take turns, so that one's weights are worked out beside the other's products: both at once would
+                // finish together and leave the matrix unit idle together.
+                const uint32_t k = t - t0;
+                if (!(t > t0 && t - 1 >= from[x] && t - 1 < to[x])) fine = fine && tc5::wait_warp(&my_turn[x], (k + x + 1) & 1, given_up, &g_status);
+                if (t < t1) scores(t);
+                if (fine && tc5::elect()) tc5::arrive(&my_turn[x ^ 1]);
+            }
             // keys and values take turns in the ring
             sv = sk + 1;
             v_turn = k_turn;
@@ -388,83 +397,109 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
                 tc5::before_sync();
                 __syncwarp();
                 if (lane == 0) tc5::arrive(&s_read[x]);
+                if (turn > 0) {  // the last tile's weights have been taken, and its sums are there
+                    fine = tc5::wait_warp(&o_done[x], (turn - 1) & 1, given_up, &g_status);
+                    if (!fine) break;
+                    tc5::after_sync();
+                }
             }
-            // 32 keys at a time: seen by every row, by none, or by some
             const int j0 = base + t * kKeys;
-            bool none[4];
-            float most = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const int b = j0 + n * 32, e = b + 32;
-                none[n] = first_lo >= e || last_hi <= b;
-                if (none[n]) continue;
-                if (last_lo > b || first_hi < e) {
-                    const int lo_n = max(my_lo - b, 0), hi_n = min(my_hi - b, 32);
-                    const uint32_t keep = hi_n <= lo_n ? 0u : (0xffffffffu >> (32 - (hi_n - lo_n))) << lo_n;
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (!(keep >> c & 1)) s[n][c] = 0xff800000u;  // -infinity
-                }
-                float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    top[0] = max3(top[0], __uint_as_float(s[n][c]), __uint_as_float(s[n][c + 1]));
-                    top[1] = max3(top[1], __uint_as_float(s[n][c + 2]), __uint_as_float(s[n][c + 3]));
-                }
-                most = max3(most, top[0], top[1]);
-            }
-            float fade = 1.f;
-            if (most > m) {
-                if (m == -INFINITY) {
-                    m = most;
-                } else if ((most - m) * a.c > kLazy) {
-                    fade = ex2((m - most) * a.c);
-                    m = most;
-                }
-            }
-            if (S::kApart && turn > 0) {  // the last tile's weights have been taken, and its sums are there
-                fine = tc5::wait_warp(&o_done[x], (turn - 1) & 1, given_up, &g_status);
-                if (!fine) break;
-                tc5::after_sync();
-            }
-            if (__any_sync(0xffffffffu, fade != 1.f)) {
-                // the sums so far are all there: where P has S's place, this tile's S came after the last tile's O
-                l *= fade;
-#pragma unroll 1
-                for (int n = 0; n < DP; n += 16) {
-                    uint32_t o[16];
-                    tc5::ld16(o, o_at + n);
-                    tc5::ld_wait(o);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                    tc5::st16(o_at + n, o);
-                }
-            }
-            const float shift = m == -INFINITY ? 0.f : -m * a.c;
-            const float2 c2 = {a.c, a.c}, shift2 = {shift, shift};
+            const bool whole = last_lo <= j0 && first_hi >= j0 + kKeys;  // every row sees every key
+            float shift = -m * a.c;
+            const float2 c2 = {a.c, a.c};
             float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            // 32 weights, two at a time, and what else there is to do beside them
+            const auto weights = [&](int n, auto beside) {
+                const float2 shift2 = {shift, shift};
                 uint32_t p[16];
-                if (none[n]) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) p[e] = 0;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float2 z = fma2({__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1])}, c2, shift2);
-                        z.x = ex2(z.x);
-                        z.y = ex2(z.y);
-                        sum[e & 1] = add2(sum[e & 1], z);
-                        p[e] = pack<T>(z.x, z.y);
-                    }
+                for (int e = 0; e < 16; ++e) {
+                    float2 z = fma2({__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1])}, c2, shift2);
+                    z.x = ex2(z.x);
+                    z.y = ex2(z.y);
+                    sum[e & 1] = add2(sum[e & 1], z);
+                    p[e] = pack<T>(z.x, z.y);
+                    beside(e);
                 }
                 tc5::st16(p_at + n * 16, p);
-                if (n == 1) {
-                    tc5::st_wait();
-                    tc5::before_sync();
-                    __syncwarp();
-                    if (lane == 0) tc5::arrive(&p_first[x]);
+            };
+            // In a tile that every row sees all of, the first half of the weights is worked out with the maximum there was before, and the tile's
+            // own maximum beside it.  It hardly ever outgrows the other by as much as it may.
+            bool careful = !whole || turn == 0;
+            if (!careful) {
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    weights(n, [&](int e) {
+                        top[0] = max3(top[0], __uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1]));
+                        top[1 + n] = max3(top[1 + n], __uint_as_float(s[n + 2][e * 2]), __uint_as_float(s[n + 2][e * 2 + 1]));
+                    });
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                careful = __any_sync(0xffffffffu, !((most - m) * a.c <= kLazy));
+            }
+            bool none[4] = {false, false, false, false};
+            if (careful) {
+                float most = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {  // 32 keys at a time: seen by none, by every row or by some
+                    const int b = j0 + n * 32, e = b + 32;
+                    none[n] = first_lo >= e || last_hi <= b;
+                    if (none[n]) continue;
+                    const int lo_n = max(my_lo - b, 0), hi_n = min(my_hi - b, 32);
+                    const uint32_t keep = hi_n <= lo_n ? 0u : (0xffffffffu >> (32 - (hi_n - lo_n))) << lo_n;
+                    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        if (!(keep >> c & 1)) s[n][c] = 0xff800000u;  // -infinity
+                        top[c & 1] = fmaxf(top[c & 1], __uint_as_float(s[n][c]));
+                    }
+                    most = max3(most, top[0], top[1]);
+                }
+                float fade = 1.f;
+                if (most > m) {
+                    if (m == -INFINITY) {
+                        m = most;
+                    } else if ((most - m) * a.c > kLazy) {
+                        fade = ex2((m - most) * a.c);
+                        m = most;
+                    }
+                }
+                if (__any_sync(0xffffffffu, fade != 1.f)) {
+                    // the sums so far are all there: where P has S's place, this tile's S came after the last tile's O
+                    l *= fade;
+#pragma unroll 1
+                    for (int n = 0; n < DP; n += 16) {
+                        uint32_t o[16];
+                        tc5::ld16(o, o_at + n);
+                        tc5::ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                        tc5::st16(o_at + n, o);
+                    }
+                }
+                shift = m == -INFINITY ? 0.f : -m * a.c;
+                sum[0] = sum[1] = {0.f, 0.f};
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    if (none[n]) {
+                        const uint32_t p[16] = {};
+                        tc5::st16(p_at + n * 16, p);
+                    } else {
+                        weights(n, [](int) {});
+                    }
+                }
+            }
+            tc5::st_wait();
+            tc5::before_sync();
+            __syncwarp();
+            if (lane == 0) tc5::arrive(&p_first[x]);
+#pragma unroll
+            for (int n = 2; n < 4; ++n) {
+                if (none[n]) {
+                    const uint32_t p[16] = {};
+                    tc5::st16(p_at + n * 16, p);
+                } else {
+                    weights(n, [](int) {});
                 }
             }
             sum[0] = add2(sum[0], sum[1]);
