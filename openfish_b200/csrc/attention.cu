@@ -4,18 +4,16 @@
 //
 // in one pass over the keys: m_i is a running maximum, and what has been summed is scaled when it moves.
 //
-// A block takes 256 rows of one sequence and key head.  The query heads that share a key head are rows next to each
-// other (row r is query r / g, head r % g of the group), so that grouped heads and single tokens fill the same tiles and
-// a key is read once for all of them.  The rows are two halves of 128, and the keys come in tiles of 128:
+// A block takes 128 rows of one sequence and key head against the keys in tiles of 64; several blocks share an SM.  The
+// query heads that share a key head are rows next to each other (row r is query r / g, head r % g of the group), so
+// that grouped heads and single tokens fill the same tiles and a key is read once for all of them.
 //
-//   warps 0-3, 4-7   the softmax of the first and second half, a thread to a row
-//   warp 8           asynchronous copies of the keys' and values' tiles into a ring in shared memory
-//   warps 9, 10      a half's matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there
+//   warps 0-3  the softmax, a thread to a row; the first of them also starts the copies of the keys' and values' tiles
+//   warp 4     the matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there, in S's place
 //
-// Heads of up to 64 have room for P beside S in tensor memory: the next tile's S is formed while this tile's weights are
-// worked out.  With larger heads P takes the place of its S, and a half's products follow one another: the first 64
-// keys' O += P V while the others' weights are still worked out, the rest, S of the next tile.  The matrix unit has the other
-// half's products in the meantime.
+// Tensor memory and registers decide how many blocks there are to an SM, and only other blocks' work fills the waits between a
+// tile's steps.  Heads of up to 64: S and O take 128 columns, four blocks.  Heads of up to 128: O alone takes that, so two
+// blocks, each with two S in turn: the next tile's S is formed while this tile's weights are worked out.
 #include <math.h>
 #include <stdint.h>
 
@@ -26,9 +24,9 @@ namespace {
 
 __device__ int g_status;  // of the kernels on this device: a wait that ran out
 
-constexpr int kHalf = 128;  // rows of a half
-constexpr int kKeys = 128;  // keys of a tile
-constexpr int kThreads = 352;
+constexpr int kRows = 128;  // of a block
+constexpr int kKeys = 64;   // of a tile
+constexpr int kThreads = 160;
 constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled: weights up to 256
 
 struct Args {
@@ -39,7 +37,7 @@ struct Args {
     long long q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head, out_stride_row, out_stride_head;
     int q_rows, k_rows, q_heads, kv_heads, group, head_dim, sequences, max_q, max_k, left, right;
     uint32_t group_mul, group_shift;  // r / group = (mulhi(r, group_mul) + r) >> group_shift for r < 2^30
-    int tiles, splits;  // of 256 rows of the longest sequence; pieces of a tile's keys
+    int tiles, splits;  // blocks of rows to the longest sequence; pieces of a block's keys
     float c;
 };
 
@@ -100,13 +98,13 @@ __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
 
 template <int DP>
 struct Shape {
-    static constexpr int kChunks = DP / 64;                   // of 64 elements, 128 bytes
-    static constexpr int kTileBytes = kChunks * 128 * 128;    // 128 rows
-    static constexpr int kStages = DP == 64 ? 10 : 5;
-    static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes + (2 * kStages + 14) * 8 + 16;
-    // columns of tensor memory: two S, two O, and two P where there is room
-    static constexpr bool kApart = DP == 64;
-    static constexpr int kOut = 2 * kKeys, kWeights = kApart ? kOut + 2 * DP : 0, kWeightsStep = kApart ? kKeys / 2 : kKeys;
+    static constexpr int kBuffers = DP == 64 ? 1 : 2, kBlocks = DP == 64 ? 4 : 2;  // S at a time; blocks to an SM
+    static constexpr int kChunks = DP / 64;                                        // of 64 elements, 128 bytes
+    static constexpr int kQueryBytes = kChunks * kRows * 128, kTileBytes = kChunks * kKeys * 128;
+    // A tile of keys has been read when its S is there; one of values when S is there that comes after its O += P V.
+    static constexpr int kKeyStages = 2, kValueStages = kBuffers + 1;
+    static constexpr int kBytes = kQueryBytes + (kKeyStages + kValueStages) * kTileBytes + (kKeyStages + kValueStages + 3 * kBuffers + 1) * 8 + 8;
+    static constexpr int kColumns = kBuffers * kKeys + DP, kOut = kBuffers * kKeys;  // of tensor memory, a power of two; O's first
 };
 
 // One row again, by a warp, straight from its definition and reading only the keys that the row sees.  A matrix
@@ -150,215 +148,152 @@ __device__ __noinline__ float2 redo_row(const T *q, const T *k, const T *v, long
 }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
-                                                                const __grid_constant__ CUtensorMap map_v) {
+__global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
+                                                                                 const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<DP>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- which rows, which keys.  The last rows come first: under a causal mask they have the most keys.
     const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
     const int pairs = a.kv_heads * a.sequences;
-    const int kh = rest % pairs % a.kv_heads, seq = rest % pairs / a.kv_heads, tile = a.tiles - 1 - rest / pairs;
+    const int kh = rest % pairs % a.kv_heads, seq = rest % pairs / a.kv_heads, block = a.tiles - 1 - rest / pairs;
     int q0, nq, k0, nk;
     span(a.q_start, a.q_used, seq, a.q_rows, a.max_q, &q0, &nq);
     span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
-    const int rows = nq * a.group, r0 = tile * 2 * kHalf;
+    const int rows = nq * a.group, r0 = block * kRows;
     if (r0 >= rows) return;
-    int lo[2], hi[2];  // the keys that a half's rows see between them
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int first = r0 + x * kHalf, last = min(first + kHalf, rows) - 1;
-        lo[x] = hi[x] = 0;
-        if (first < rows) {
-            int unused;
-            window(a, by_group(a, first), nq, nk, &lo[x], &unused);
-            window(a, by_group(a, last), nq, nk, &unused, &hi[x]);
-            if (hi[x] <= lo[x]) lo[x] = hi[x] = 0;
-        }
-    }
-    const int base = hi[1] <= lo[1] ? lo[0] : hi[0] <= lo[0] ? lo[1] : min(lo[0], lo[1]);
-    const int tiles = (max(max(hi[0], hi[1]) - base, 0) + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
-    const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
-    int from[2], to[2];  // each half's tiles
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        from[x] = to[x] = 0;
-        if (hi[x] > lo[x]) {
-            from[x] = max(t0, (lo[x] - base) / kKeys);
-            to[x] = min(t1, (hi[x] - base + kKeys - 1) / kKeys);
-            if (to[x] <= from[x]) from[x] = to[x] = 0;
-        }
-    }
+    int lo, hi, unused;  // the keys that the rows see between them
+    window(a, by_group(a, r0), nq, nk, &lo, &unused);
+    window(a, by_group(a, min(r0 + kRows, rows) - 1), nq, nk, &unused, &hi);
+    const int tiles = (max(hi - lo, 0) + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
+    const int first = min(split * per, tiles), count = min(per, tiles - first);  // this split's tiles
+    const int base = lo + first * kKeys;                                         // and its first key
 
-    extern __shared__ uint8_t raw[];
-    uint8_t *const q_tiles = raw + ((1024 - (tc5::smem_u32(raw) & 1023)) & 1023);
-    uint8_t *const ring = q_tiles + 2 * S::kTileBytes;
-    uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kTileBytes), *const empty = full + S::kStages;
-    uint64_t *const q_ready = empty + S::kStages, *const s_full = q_ready + 2, *const s_read = s_full + 2, *const p_first = s_read + 2;
-    uint64_t *const p_ready = p_first + 2, *const o_done = p_ready + 2, *const my_turn = o_done + 2;
-    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(my_turn + 2);
+    extern __shared__ __align__(1024) uint8_t q_tile[];  // the swizzle counts from 1024-byte boundaries
+    uint8_t *const k_tiles = q_tile + S::kQueryBytes, *const v_tiles = k_tiles + S::kKeyStages * S::kTileBytes;
+    uint64_t *const k_full = reinterpret_cast<uint64_t *>(v_tiles + S::kValueStages * S::kTileBytes), *const v_full = k_full + S::kKeyStages;
+    uint64_t *const s_full = v_full + S::kValueStages, *const p_ready = s_full + S::kBuffers, *const q_ready = p_ready + S::kBuffers;
+    uint64_t *const o_done = q_ready + 1;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_done + S::kBuffers);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
+    const auto load_keys = [&](int t) {
+        uint64_t *const bar = &k_full[t % S::kKeyStages];
+        ofd::mbar_arrive_expect_tx(bar, S::kTileBytes);
+#pragma unroll
+        for (int d = 0; d < S::kChunks; ++d)
+            tc5::load_3d(k_tiles + t % S::kKeyStages * S::kTileBytes + d * kKeys * 128, &map_k, d * 64, kh, k0 + base + t * kKeys, bar);
+    };
+    const auto load_values = [&](int t) {
+        uint64_t *const bar = &v_full[t % S::kValueStages];
+        ofd::mbar_arrive_expect_tx(bar, S::kTileBytes);
+#pragma unroll
+        for (int d = 0; d < S::kChunks; ++d)
+            tc5::load_3d(v_tiles + t % S::kValueStages * S::kTileBytes + d * kKeys * 128, &map_v, d * 64, kh, k0 + base + t * kKeys, bar);
+    };
     if (threadIdx.x == 0) {
         *given_up = 0;
-        for (int i = 0; i < S::kStages; ++i) {
-            ofd::mbar_init(&full[i], 1);
-            ofd::mbar_init(&empty[i], 2);
+        for (int i = 0; i < S::kKeyStages; ++i) ofd::mbar_init(&k_full[i], 1);
+        for (int i = 0; i < S::kValueStages; ++i) ofd::mbar_init(&v_full[i], 1);
+        for (int i = 0; i < S::kBuffers; ++i) {
+            ofd::mbar_init(&s_full[i], 1);
+            ofd::mbar_init(&p_ready[i], 4);
+            ofd::mbar_init(&o_done[i], 1);
         }
-        for (int x = 0; x < 2; ++x) {
-            ofd::mbar_init(&q_ready[x], 4);
-            ofd::mbar_init(&s_full[x], 1);
-            ofd::mbar_init(&s_read[x], 4);
-            ofd::mbar_init(&p_first[x], 4);
-            ofd::mbar_init(&p_ready[x], 4);
-            ofd::mbar_init(&o_done[x], 1);
-            ofd::mbar_init(&my_turn[x], 1);
-        }
+        ofd::mbar_init(q_ready, 4);
         ofd::mbar_fence_init();
-        tc5::prefetch_map(&map_k);
-        tc5::prefetch_map(&map_v);
+        if (count > 0) {
+            load_keys(0);
+            load_values(0);
+            if (count > 1) load_keys(1);
+        }
     }
-    if (warp == 9) tc5::tmem_alloc<1>(tmem_slot, 512);
+    if (warp == 4) tc5::tmem_alloc<1>(tmem_slot, S::kColumns);
     tc5::before_sync();
     __syncthreads();
     tc5::after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 8) {
-        if (lane == 0) {
-            int i = 0;  // tiles of the ring, in the order keys, values, keys, ...
-            bool fine = true;
-            for (int t = t0; t < t1 && fine; ++t) {
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv, ++i) {
-                    const int s = i % S::kStages;
-                    fine = fine && tc5::wait(&empty[s], ((i / S::kStages) & 1) ^ 1, given_up, &g_status);
-                    if (!fine) break;
-                    ofd::mbar_arrive_expect_tx(&full[s], S::kTileBytes);
-#pragma unroll
-                    for (int d = 0; d < S::kChunks; ++d)
-                        tc5::load_3d(ring + s * S::kTileBytes + d * 16384, kv ? &map_v : &map_k, d * 64, kh, k0 + base + t * kKeys, &full[s]);
-                }
-            }
-            if (!fine) ofd::mbar_drain_bounded(full, S::kStages, i, ofd::kDefaultWaitLimitNs);
-        }
-    } else if (warp >= 9) {
+    if (warp == 4) {
         // The instructions are issued one after the other by one thread, whose own pace counts: descriptors are sums with
         // constants, loops are unrolled.
-        const int x = warp - 9;
         constexpr bool bf16 = __is_same(T, __nv_bfloat16);
         constexpr uint32_t idesc_s = tc5::idesc_f16(128, kKeys, bf16, false), idesc_o = tc5::idesc_f16(128, DP, bf16, true);
-        const uint64_t q_desc = tc5::desc_k_major(tc5::smem_u32(q_tiles) + x * S::kTileBytes), k_desc = tc5::desc_k_major(tc5::smem_u32(ring));
-        const uint64_t v_desc = tc5::desc_mn_major(tc5::smem_u32(ring), 16384);
-        const uint32_t s_at = tmem + x * kKeys, o_at = tmem + S::kOut + x * DP, p_at = tmem + S::kWeights + x * S::kWeightsStep;
-        int sk = 0, sv = 0;               // the ring's places of tile t's keys and of tile t - 1's values
-        uint32_t k_turn = 0, v_turn = 0;  // and their turns
-        uint32_t turn = 0;                // tiles of this half whose values have been taken
+        const uint64_t q_desc = tc5::desc_k_major(tc5::smem_u32(q_tile)), k_desc = tc5::desc_k_major(tc5::smem_u32(k_tiles));
+        const uint64_t v_desc = tc5::desc_mn_major(tc5::smem_u32(v_tiles), kKeys * 128);
         bool fine = true;
-        const auto scores = [&](int t) {  // S = Q K^T of tile t; true if there is none
-            fine = fine && tc5::wait_warp(&full[sk], k_turn, given_up, &g_status);
-            if (fine && t >= from[x] && t < to[x]) {
-                if (t == from[x]) fine = tc5::wait_warp(&q_ready[x], 0, given_up, &g_status);
-                else if (S::kApart) fine = tc5::wait_warp(&s_read[x], (t - from[x] - 1) & 1, given_up, &g_status);
-                tc5::after_sync();
-                const uint64_t kd = k_desc + (uint32_t)(sk * (S::kTileBytes >> 4));
-                if (fine && tc5::elect()) {
+        const auto scores = [&](int t) {  // S = Q K^T of tile t
+            fine = fine && tc5::wait_warp(&k_full[t % S::kKeyStages], t / S::kKeyStages & 1, given_up, &g_status);
+            tc5::after_sync();
+            const uint32_t s_at = tmem + t % S::kBuffers * kKeys;
+            const uint64_t kd = k_desc + (uint32_t)(t % S::kKeyStages * (S::kTileBytes >> 4));
+            if (fine && tc5::elect()) {
 #pragma unroll
-                    for (int n = 0; n < DP / 16; ++n) {
-                        const uint32_t at = ((n >> 2) * 16384 + (n & 3) * 32) >> 4;
-                        tc5::mma_f16(s_at, q_desc + at, kd + at, idesc_s, n > 0);
-                    }
-                    tc5::commit(&s_full[x]);
-                }
+                for (int n = 0; n < DP / 16; ++n)
+                    tc5::mma_f16(s_at, q_desc + ((n >> 2) * (kRows * 128 >> 4) + (n & 3) * 2), kd + ((n >> 2) * (kKeys * 128 >> 4) + (n & 3) * 2), idesc_s, n > 0);
+                tc5::commit(&s_full[t % S::kBuffers]);
             }
-            if (fine && tc5::elect()) tc5::commit(&empty[sk]);
         };
-        const auto sums = [&](int t) {  // O += P V of tile t
-            fine = fine && tc5::wait_warp(&full[sv], v_turn, given_up, &g_status);
-            if (fine && t >= from[x] && t < to[x]) {
-                const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
-                if (valid & 15) {
-                    // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
-                    const int count = 16 - (valid & 15);
-                    for (int n = lane; n < count * 8 * S::kChunks; n += 32) {
-                        const int d = n / (count * 8), in = n % (count * 8);
-                        *reinterpret_cast<uint4 *>(ring + sv * S::kTileBytes + d * 16384 + valid * 128 + in * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    tc5::fence_async();
-                    __syncwarp();
+        int sv = 0;  // the place of tile t's values, and its turn
+        uint32_t v_turn = 0;
+        if (count > 0) {
+            fine = tc5::wait_warp(q_ready, 0, given_up, &g_status);
+            scores(0);
+        }
+        for (int t = 0; t < count && fine; ++t) {
+            if (S::kBuffers == 2 && t + 1 < count) scores(t + 1);
+            fine = fine && tc5::wait_warp(&v_full[sv], v_turn, given_up, &g_status);
+            const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
+            if (fine && (valid & 15)) {
+                // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
+                const int behind = 16 - (valid & 15);
+                for (int n = lane; n < behind * 8 * S::kChunks; n += 32) {
+                    const int d = n / (behind * 8), in = n % (behind * 8);
+                    *reinterpret_cast<uint4 *>(v_tiles + sv * S::kTileBytes + d * kKeys * 128 + valid * 128 + in * 16) = make_uint4(0, 0, 0, 0);
                 }
-                const uint64_t vd = v_desc + (uint32_t)(sv * (S::kTileBytes >> 4));
-                fine = tc5::wait_warp(&p_first[x], turn & 1, given_up, &g_status);
-                tc5::after_sync();
-                if (fine && tc5::elect()) {
-                    if (steps >= 4) {
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, turn > 0 || n > 0);
-                    } else {
-                        for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, turn > 0 || n > 0);
-                    }
-                }
-                fine = fine && tc5::wait_warp(&p_ready[x], turn & 1, given_up, &g_status);
-                if (!S::kApart) fine = fine && tc5::wait_warp(&my_turn[x], (t + 1 - t0 + x + 1) & 1, given_up, &g_status);
-                tc5::after_sync();
-                if (fine && tc5::elect()) {
-                    if (steps == 8) {
-#pragma unroll
-                        for (int n = 4; n < 8; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, true);
-                    } else {
-                        for (int n = 4; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, true);
-                    }
-                    if (S::kApart || t + 1 == to[x]) tc5::commit(&o_done[x]);
-                }
-                ++turn;
+                tc5::fence_async();
+                __syncwarp();
             }
-            if (fine && tc5::elect()) tc5::commit(&empty[sv]);
-        };
-        for (int t = t0; t <= t1 && fine; ++t) {
-            if (S::kApart && t < t1) scores(t);
-            if (t > t0) sums(t - 1);
-            if (!S::kApart) {
-                // The halves take turns, so that one's weights are worked out beside the other's products: both at once would
-                // finish together and leave the matrix unit idle together.
-                const uint32_t k = t - t0;
-                if (!(t > t0 && t - 1 >= from[x] && t - 1 < to[x])) fine = fine && tc5::wait_warp(&my_turn[x], (k + x + 1) & 1, given_up, &g_status);
-                if (t < t1) scores(t);
-                if (fine && tc5::elect()) tc5::arrive(&my_turn[x ^ 1]);
+            const uint64_t vd = v_desc + (uint32_t)(sv * (S::kTileBytes >> 4));
+            const uint32_t o_at = tmem + S::kOut, p_at = tmem + t % S::kBuffers * kKeys;
+            fine = fine && tc5::wait_warp(&p_ready[t % S::kBuffers], t / S::kBuffers & 1, given_up, &g_status);
+            tc5::after_sync();
+            if (fine && tc5::elect()) {
+                if (steps == 4) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, t > 0 || n > 0);
+                } else {
+                    for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, t > 0 || n > 0);
+                }
+                if (S::kBuffers == 2 || t + 1 == count) tc5::commit(&o_done[t % S::kBuffers]);
             }
-            // keys and values take turns in the ring
-            sv = sk + 1;
-            v_turn = k_turn;
-            if (sv == S::kStages) sv = 0, v_turn ^= 1;
-            sk = sv + 1;
-            k_turn = v_turn;
-            if (sk == S::kStages) sk = 0, k_turn ^= 1;
             __syncwarp();
+            if (S::kBuffers == 1 && t + 1 < count) scores(t + 1);
+            if (++sv == S::kValueStages) sv = 0, v_turn ^= 1;
         }
         if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
-            tc5::commit(&o_done[x]);
-            ofd::mbar_land(&o_done[x], 0, 0, ofd::kDefaultWaitLimitNs);
+            tc5::commit(o_done);
+            ofd::mbar_land(o_done, 0, 0, ofd::kDefaultWaitLimitNs);
         }
     } else {
-        const int x = warp >> 2;
-        const int row = (warp & 3) * 32 + lane;  // of the half, and lane of tensor memory
-        const int r = r0 + x * kHalf + row, i = by_group(a, r), head = kh * a.group + r - i * a.group;
-        const bool there = r < rows;
-        const bool warp_there = r0 + x * kHalf + (warp & 3) * 32 < rows;
-        // ---- this half's queries into shared memory, pieces of 16 bytes; zeros where there are none
-        if (from[x] < to[x]) {
+        const int row = warp * 32 + lane;  // of the block, and lane of tensor memory
+        const int r = r0 + row, i = by_group(a, r), head = kh * a.group + r - i * a.group;
+        const bool there = r < rows, warp_there = r0 + warp * 32 < rows;
+        // ---- the queries into shared memory, pieces of 16 bytes; zeros where there are none
+        if (count > 0) {
             constexpr int kPieces = DP / 8;
 #pragma unroll 4
-            for (int n = threadIdx.x & 127; n < kHalf * kPieces; n += 128) {
-                const int qr = n / kPieces, p = n % kPieces, rr = r0 + x * kHalf + qr, ri = by_group(a, rr);
+            for (int n = threadIdx.x; n < kRows * kPieces; n += 128) {
+                const int qr = n / kPieces, p = n % kPieces, rr = r0 + qr, ri = by_group(a, rr);
                 uint4 val = make_uint4(0, 0, 0, 0);
                 if (rr < rows && p * 8 < a.head_dim)
                     val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(q0 + ri) * a.q_stride_row +
                                                            (kh * a.group + rr - ri * a.group) * a.q_stride_head + p * 8);
-                *reinterpret_cast<uint4 *>(q_tiles + x * S::kTileBytes + (p >> 3) * 16384 + qr * 128 + (((p & 7) ^ (qr & 7)) << 4)) = val;
+                *reinterpret_cast<uint4 *>(q_tile + (p >> 3) * kRows * 128 + qr * 128 + (((p & 7) ^ (qr & 7)) << 4)) = val;
             }
             tc5::fence_async();
             __syncwarp();
-            if (lane == 0) tc5::arrive(&q_ready[x]);
+            if (lane == 0) tc5::arrive(q_ready);
         }
         // ---- the keys this row sees, and between them the first and the last row of the warp (rows that are not there
         // are given the last row's)
@@ -367,156 +302,133 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
         const int first_lo = __shfl_sync(0xffffffffu, my_lo, 0), first_hi = __shfl_sync(0xffffffffu, my_hi, 0);
         const int last_lo = __shfl_sync(0xffffffffu, my_lo, 31), last_hi = __shfl_sync(0xffffffffu, my_hi, 31);
         float m = -INFINITY, l = 0.f;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + x * kKeys, o_at = tmem + lanes + S::kOut + x * DP;
-        const uint32_t p_at = tmem + lanes + S::kWeights + x * S::kWeightsStep;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16, o_at = tmem + lanes + S::kOut;
         bool fine = true;
-        int turn = 0;
-        for (int t = from[x]; t < to[x]; ++t, ++turn) {
-            fine = tc5::wait_warp(&s_full[x], turn & 1, given_up, &g_status);
+        for (int t = 0; t < count; ++t) {
+            const int buffer = t % S::kBuffers;
+            fine = tc5::wait_warp(&s_full[buffer], t / S::kBuffers & 1, given_up, &g_status);
             if (!fine) break;
             tc5::after_sync();
-            if (!warp_there) {  // nothing but rows that are not there: their weights are whatever lies in the place
-                __syncwarp();
-                if (S::kApart && lane == 0) tc5::arrive(&s_read[x]);
-                // (not before the other warps' weights of the last tile have been taken: an arrival counts for the turn it finds)
-                if (S::kApart && turn > 0) fine = tc5::wait_warp(&o_done[x], (turn - 1) & 1, given_up, &g_status);
-                if (!fine) break;
-                if (lane == 0) {
-                    tc5::arrive(&p_first[x]);
-                    tc5::arrive(&p_ready[x]);
-                }
-                continue;
+            if (threadIdx.x == 0) {  // the tiles that have been read make room for others
+                if (t + 1 < count) load_values(t + 1);
+                if (t + 2 < count) load_keys(t + 2);
             }
-            uint32_t s[4][32];
+            __syncwarp();
+            if (warp_there) {  // (else nothing but rows that are not there: their weights are whatever lies in the place)
+                const uint32_t s_at = tmem + lanes + buffer * kKeys;
+                const int j0 = base + t * kKeys;
+                float shift = -m * a.c;
+                const float2 c2 = {a.c, a.c};
+                float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                uint32_t s[2][32], p[2][16];
+                // 32 weights, two at a time, and what else there is to do beside them
+                const auto weights = [&](int n, auto beside) {
+                    const float2 shift2 = {shift, shift};
 #pragma unroll
-            for (int n = 0; n < 4; ++n) tc5::ld32(s[n], s_at + n * 32);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) tc5::ld_wait(s[n]);
-            if (S::kApart) {
-                tc5::before_sync();
-                __syncwarp();
-                if (lane == 0) tc5::arrive(&s_read[x]);
-                if (turn > 0) {  // the last tile's weights have been taken, and its sums are there
-                    fine = tc5::wait_warp(&o_done[x], (turn - 1) & 1, given_up, &g_status);
-                    if (!fine) break;
-                    tc5::after_sync();
-                }
-            }
-            const int j0 = base + t * kKeys;
-            const bool whole = last_lo <= j0 && first_hi >= j0 + kKeys;  // every row sees every key
-            float shift = -m * a.c;
-            const float2 c2 = {a.c, a.c};
-            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-            // 32 weights, two at a time, and what else there is to do beside them
-            const auto weights = [&](int n, auto beside) {
-                const float2 shift2 = {shift, shift};
-                uint32_t p[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float2 z = fma2({__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1])}, c2, shift2);
-                    z.x = ex2(z.x);
-                    z.y = ex2(z.y);
-                    sum[e & 1] = add2(sum[e & 1], z);
-                    p[e] = pack<T>(z.x, z.y);
-                    beside(e);
-                }
-                tc5::st16(p_at + n * 16, p);
-            };
-            // In a tile that every row sees all of, the first half of the weights is worked out with the maximum there was before, and the tile's
-            // own maximum beside it.  It hardly ever outgrows the other by as much as it may.
-            bool careful = !whole || turn == 0;
-            if (!careful) {
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    weights(n, [&](int e) {
-                        top[0] = max3(top[0], __uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1]));
-                        top[1 + n] = max3(top[1 + n], __uint_as_float(s[n + 2][e * 2]), __uint_as_float(s[n + 2][e * 2 + 1]));
-                    });
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                careful = __any_sync(0xffffffffu, !((most - m) * a.c <= kLazy));
-            }
-            bool none[4] = {false, false, false, false};
-            if (careful) {
-                float most = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {  // 32 keys at a time: seen by none, by every row or by some
-                    const int b = j0 + n * 32, e = b + 32;
-                    none[n] = first_lo >= e || last_hi <= b;
-                    if (none[n]) continue;
-                    const int lo_n = max(my_lo - b, 0), hi_n = min(my_hi - b, 32);
-                    const uint32_t keep = hi_n <= lo_n ? 0u : (0xffffffffu >> (32 - (hi_n - lo_n))) << lo_n;
+                    for (int e = 0; e < 16; ++e) {
+                        float2 z = fma2({__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1])}, c2, shift2);
+                        z.x = ex2(z.x);
+                        z.y = ex2(z.y);
+                        sum[e & 1] = add2(sum[e & 1], z);
+                        p[n][e] = pack<T>(z.x, z.y);
+                        beside(e);
+                    }
+                };
+                tc5::ld32(s[0], s_at);
+                tc5::ld32(s[1], s_at + 32);
+                tc5::ld_wait(s[0]);
+                tc5::ld_wait(s[1]);
+                // In a tile that every row sees all of, the weights are worked out with the maximum there was before, and
+                // the tile's own maximum beside them.  It hardly ever outgrows the other by as much as it may.
+                bool careful = t == 0 || last_lo > j0 || first_hi < j0 + kKeys;
+                if (!careful) {
                     float top[2] = {-INFINITY, -INFINITY};
+                    weights(0, [&](int e) {
+                        top[0] = max3(top[0], __uint_as_float(s[0][e * 2]), __uint_as_float(s[0][e * 2 + 1]));
+                        top[1] = max3(top[1], __uint_as_float(s[1][e * 2]), __uint_as_float(s[1][e * 2 + 1]));
+                    });
+                    weights(1, [](int) {});
+                    careful = __any_sync(0xffffffffu, !((fmaxf(top[0], top[1]) - m) * a.c <= kLazy));
+                    if (careful) {
+                        tc5::ld32(s[0], s_at);
+                        tc5::ld32(s[1], s_at + 32);
+                        tc5::ld_wait(s[0]);
+                        tc5::ld_wait(s[1]);
+                    }
+                }
+                if (careful) {
+                    float most = -INFINITY;
+                    bool none[2];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        if (!(keep >> c & 1)) s[n][c] = 0xff800000u;  // -infinity
-                        top[c & 1] = fmaxf(top[c & 1], __uint_as_float(s[n][c]));
+                    for (int n = 0; n < 2; ++n) {  // 32 keys at a time: seen by none of the rows or by some
+                        const int b = j0 + n * 32;
+                        none[n] = first_lo >= b + 32 || last_hi <= b;
+                        if (none[n]) continue;
+                        const int lo_n = max(my_lo - b, 0), hi_n = min(my_hi - b, 32);
+                        const uint32_t keep = hi_n <= lo_n ? 0u : (0xffffffffu >> (32 - (hi_n - lo_n))) << lo_n;
+                        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            if (!(keep >> c & 1)) s[n][c] = 0xff800000u;  // -infinity
+                            top[c & 1] = fmaxf(top[c & 1], __uint_as_float(s[n][c]));
+                        }
+                        most = max3(most, top[0], top[1]);
                     }
-                    most = max3(most, top[0], top[1]);
-                }
-                float fade = 1.f;
-                if (most > m) {
-                    if (m == -INFINITY) {
-                        m = most;
-                    } else if ((most - m) * a.c > kLazy) {
-                        fade = ex2((m - most) * a.c);
-                        m = most;
+                    float fade = 1.f;
+                    if (most > m) {
+                        if (m == -INFINITY) {
+                            m = most;
+                        } else if ((most - m) * a.c > kLazy) {
+                            fade = ex2((m - most) * a.c);
+                            m = most;
+                        }
                     }
-                }
-                if (__any_sync(0xffffffffu, fade != 1.f)) {
-                    // the sums so far are all there: where P has S's place, this tile's S came after the last tile's O
-                    l *= fade;
+                    if (__any_sync(0xffffffffu, fade != 1.f)) {
+                        // the sums so far: with one S they are there when it is
+                        if (S::kBuffers == 2) fine = tc5::wait_warp(&o_done[buffer ^ 1], (t - 1) / 2 & 1, given_up, &g_status);
+                        tc5::after_sync();
+                        l *= fade;
 #pragma unroll 1
-                    for (int n = 0; n < DP; n += 16) {
-                        uint32_t o[16];
-                        tc5::ld16(o, o_at + n);
-                        tc5::ld_wait(o);
+                        for (int n = 0; n < DP; n += 16) {
+                            uint32_t o[16];
+                            tc5::ld16(o, o_at + n);
+                            tc5::ld_wait(o);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                        tc5::st16(o_at + n, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                            tc5::st16(o_at + n, o);
+                        }
+                    }
+                    shift = m == -INFINITY ? 0.f : -m * a.c;
+                    sum[0] = sum[1] = {0.f, 0.f};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        if (none[n]) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) p[n][e] = 0;
+                        } else {
+                            weights(n, [](int) {});
+                        }
                     }
                 }
-                shift = m == -INFINITY ? 0.f : -m * a.c;
-                sum[0] = sum[1] = {0.f, 0.f};
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    if (none[n]) {
-                        const uint32_t p[16] = {};
-                        tc5::st16(p_at + n * 16, p);
-                    } else {
-                        weights(n, [](int) {});
-                    }
-                }
+                tc5::st16(s_at, p[0]);
+                tc5::st16(s_at + 16, p[1]);
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
+                tc5::st_wait();
             }
-            tc5::st_wait();
+            if (!fine) break;
             tc5::before_sync();
             __syncwarp();
-            if (lane == 0) tc5::arrive(&p_first[x]);
-#pragma unroll
-            for (int n = 2; n < 4; ++n) {
-                if (none[n]) {
-                    const uint32_t p[16] = {};
-                    tc5::st16(p_at + n * 16, p);
-                } else {
-                    weights(n, [](int) {});
-                }
-            }
-            sum[0] = add2(sum[0], sum[1]);
-            l += sum[0].x + sum[0].y;
-            tc5::st_wait();
-            tc5::before_sync();
-            __syncwarp();
-            if (lane == 0) tc5::arrive(&p_ready[x]);
+            if (lane == 0) tc5::arrive(&p_ready[buffer]);
         }
         // ---- out = O / l
-        const bool any = fine && from[x] < to[x];
+        const bool any = fine && count > 0;
         if (any) {
-            fine = tc5::wait_warp(&o_done[x], S::kApart ? (turn - 1) & 1 : 0, given_up, &g_status);
+            fine = tc5::wait_warp(&o_done[(count - 1) % S::kBuffers], S::kBuffers == 2 ? (count - 1) / 2 & 1 : 0, given_up, &g_status);
             tc5::after_sync();
         }
         if (fine && warp_there) {
-            const int in_lo = max(my_lo, base + t0 * kKeys), in_hi = min(my_hi, base + t1 * kKeys);  // of this split
+            const int in_lo = max(my_lo, base), in_hi = min(my_hi, base + count * kKeys);  // of this split
             const bool sees = there && in_hi > in_lo;
             const float back = sees ? 1.f / l : 0.f;
             const long long at = (long long)(q0 + i) * a.q_heads + head;  // of [q_rows][q_heads]
@@ -553,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
             __syncwarp();
             for (uint32_t again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
                 const int who = __ffs(again) - 1;
-                const int rr = r0 + x * kHalf + (warp & 3) * 32 + who, ii = by_group(a, rr), hh = kh * a.group + rr - ii * a.group;
+                const int rr = r0 + warp * 32 + who, ii = by_group(a, rr), hh = kh * a.group + rr - ii * a.group;
                 const int klo = __shfl_sync(0xffffffffu, in_lo, who), khi = __shfl_sync(0xffffffffu, in_hi, who);
                 const long long aa = (long long)(q0 + ii) * a.q_heads + hh;
                 const float2 ml = redo_row<T>(static_cast<const T *>(a.q) + (long long)(q0 + ii) * a.q_stride_row + hh * a.q_stride_head,
@@ -571,7 +483,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const Args a, co
     tc5::before_sync();
     __syncthreads();
     tc5::after_sync();
-    if (warp == 9) tc5::tmem_free<1>(tmem, 512);
+    if (*given_up && threadIdx.x == 0) {  // the copies under way land before the block ends
+        for (int n = 0; n < S::kKeyStages + S::kValueStages; ++n) {
+            uint64_t since = ofd::mbar_land(&k_full[n], 0, 0, ofd::kDefaultWaitLimitNs / 16);
+            ofd::mbar_land(&k_full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
+        }
+    }
+    if (warp == 4) tc5::tmem_free<1>(tmem, S::kColumns);
 }
 
 // The splits' results joined: out = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A warp to a query and head.
@@ -608,18 +526,19 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
     }
 }
 
-// Into how many pieces a tile's keys go: enough blocks to fill the SMs, two tiles of keys to a piece at least.
+// Into how many pieces a block's keys go: enough blocks to fill the SMs, four tiles of keys to a piece at least.
 int splits_for(const openfish_b200_attention_t *a, int sms) {
     const long long group = a->q_heads / a->kv_heads;
-    const long long blocks = (a->max_q * group + 2 * kHalf - 1) / (2 * kHalf) * a->kv_heads * a->sequences;
+    const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64>::kBlocks : Shape<128>::kBlocks);
+    const long long blocks = (a->max_q * group + kRows - 1) / kRows * a->kv_heads * a->sequences;
     long long keys = a->max_k;
     if (a->window_left >= 0 && a->window_right >= 0) {
-        const long long seen = (long long)a->window_left + a->window_right + 1 + 2 * kHalf / group;
+        const long long seen = (long long)a->window_left + a->window_right + 1 + kRows / group;
         if (seen < keys) keys = seen;
     }
     const long long tiles = (keys + kKeys - 1) / kKeys;
-    long long n = sms / blocks;
-    if (n > tiles / 2) n = tiles / 2;
+    long long n = room / blocks;
+    if (n > tiles / 4) n = tiles / 4;
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
 }
@@ -677,7 +596,7 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     a.group_shift = (uint32_t)bits;
     a.group_mul = (uint32_t)(((1ull << 32) * ((1ull << bits) - (unsigned)a.group)) / (unsigned)a.group + 1);
     a.c = p->scale * 1.4426950408889634f;
-    a.tiles = (int)(((long long)p->max_q * a.group + 2 * kHalf - 1) / (2 * kHalf));
+    a.tiles = (int)(((long long)p->max_q * a.group + kRows - 1) / kRows);
     a.splits = splits_for(p, sms);
     a.part_lse = static_cast<float *>(p->workspace);
     a.part = a.part_lse;

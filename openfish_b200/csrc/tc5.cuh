@@ -17,7 +17,7 @@ using ofd::smem_u32;
 
 // ---- waits.  A block's flag goes up when one of its waits has run out; from then on every wait that does not find its phase complete at once
 // returns false, every role leaves its loop, and the kernel ends in order.
-static __device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status) {
+static __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status) {
     uint64_t t0 = 0;
     for (uint32_t spin = 1;; ++spin) {
         if (mbar_try_wait(bar, parity)) return true;
