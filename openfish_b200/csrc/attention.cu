@@ -8,8 +8,9 @@
 // query heads that share a key head are rows next to each other (row r is query r / g, head r % g of the group), so
 // that grouped heads and single tokens fill the same tiles and a key is read once for all of them.
 //
-//   warps 0-3  the softmax, a thread to a row; the first of them also starts the copies of the keys' and values' tiles
-//   warp 4     the matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there, in S's place
+//   warps 0-3  the softmax, a thread to a row
+//   warp 4     the matrix instructions, S = Q K^T into tensor memory and O += P V with P read from there, in S's place; and the
+//              asynchronous copies of the keys' and values' tiles
 //
 // Tensor memory and registers decide how many blocks there are to an SM, and only other blocks' work fills the waits between a
 // tile's steps.  Heads of up to 64: S and O take 128 columns, four blocks.  Heads of up to 128: O alone takes that, so two
@@ -26,7 +27,6 @@ __device__ int g_status;  // of the kernels on this device: a wait that ran out
 
 constexpr int kRows = 128;  // of a block
 constexpr int kKeys = 64;   // of a tile
-constexpr int kThreads = 160;
 constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled: weights up to 256
 
 struct Args {
@@ -96,14 +96,26 @@ __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Two weights 2^(c s - c m) as the matrix unit takes them, added to their row's sum (before they are rounded).
+template <class T>
+__device__ __forceinline__ uint32_t weights(float u, float w, float c, float shift, float2 &sum) {
+    float2 z = fma2({u, w}, {c, c}, {shift, shift});
+    z.x = ex2(z.x);
+    z.y = ex2(z.y);
+    sum = add2(sum, z);
+    return pack<T>(z.x, z.y);
+}
+
 template <int DP>
 struct Shape {
     static constexpr int kBuffers = DP == 64 ? 1 : 2, kBlocks = DP == 64 ? 4 : 2;  // S at a time; blocks to an SM
     static constexpr int kChunks = DP / 64;                                        // of 64 elements, 128 bytes
     static constexpr int kQueryBytes = kChunks * kRows * 128, kTileBytes = kChunks * kKeys * 128;
-    // A tile of keys has been read when its S is there; one of values when S is there that comes after its O += P V.
-    static constexpr int kKeyStages = 2, kValueStages = kBuffers + 1;
-    static constexpr int kBytes = kQueryBytes + (kKeyStages + kValueStages) * kTileBytes + (kKeyStages + kValueStages + 3 * kBuffers + 1) * 8 + 8;
+    static constexpr int kKeyStages = kBuffers + 1, kValueStages = 2;
+    // a warp of its own starts the copies where registers allow one
+    static constexpr bool kCopyWarp = DP == 128;
+    static constexpr int kThreads = kCopyWarp ? 192 : 160;
+    static constexpr int kBytes = kQueryBytes + (kKeyStages + kValueStages) * kTileBytes + (2 * (kKeyStages + kValueStages) + 3 * kBuffers + 1) * 8 + 8;
     static constexpr int kColumns = kBuffers * kKeys + DP, kOut = kBuffers * kKeys;  // of tensor memory, a power of two; O's first
 };
 
@@ -148,7 +160,7 @@ __device__ __noinline__ float2 redo_row(const T *q, const T *k, const T *v, long
 }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
                                                                                  const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<DP>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -172,7 +184,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
     extern __shared__ __align__(1024) uint8_t q_tile[];  // the swizzle counts from 1024-byte boundaries
     uint8_t *const k_tiles = q_tile + S::kQueryBytes, *const v_tiles = k_tiles + S::kKeyStages * S::kTileBytes;
     uint64_t *const k_full = reinterpret_cast<uint64_t *>(v_tiles + S::kValueStages * S::kTileBytes), *const v_full = k_full + S::kKeyStages;
-    uint64_t *const s_full = v_full + S::kValueStages, *const p_ready = s_full + S::kBuffers, *const q_ready = p_ready + S::kBuffers;
+    uint64_t *const k_free = v_full + S::kValueStages, *const v_free = k_free + S::kKeyStages;
+    uint64_t *const s_full = v_free + S::kValueStages, *const p_ready = s_full + S::kBuffers, *const q_ready = p_ready + S::kBuffers;
     uint64_t *const o_done = q_ready + 1;
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_done + S::kBuffers);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -193,8 +206,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
     };
     if (threadIdx.x == 0) {
         *given_up = 0;
-        for (int i = 0; i < S::kKeyStages; ++i) ofd::mbar_init(&k_full[i], 1);
-        for (int i = 0; i < S::kValueStages; ++i) ofd::mbar_init(&v_full[i], 1);
+        for (int i = 0; i < 2 * (S::kKeyStages + S::kValueStages); ++i) ofd::mbar_init(&k_full[i], 1);
         for (int i = 0; i < S::kBuffers; ++i) {
             ofd::mbar_init(&s_full[i], 1);
             ofd::mbar_init(&p_ready[i], 4);
@@ -205,7 +217,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
         if (count > 0) {
             load_keys(0);
             load_values(0);
-            if (count > 1) load_keys(1);
+            for (int t = 1; t < S::kKeyStages && t < count; ++t) load_keys(t);
+            for (int t = 1; t < S::kValueStages && t < count; ++t) load_values(t);
         }
     }
     if (warp == 4) tc5::tmem_alloc<1>(tmem_slot, S::kColumns);
@@ -214,7 +227,21 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
     tc5::after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 4) {
+    if (S::kCopyWarp && warp == 5) {
+        if (lane == 0) {
+            bool fine = true;
+            for (int t = 0; t < count && fine; ++t) {
+                if (t + S::kKeyStages < count) {
+                    fine = tc5::wait(&k_free[t % S::kKeyStages], t / S::kKeyStages & 1, given_up, &g_status);
+                    if (fine) load_keys(t + S::kKeyStages);
+                }
+                if (fine && t + S::kValueStages < count) {
+                    fine = tc5::wait(&v_free[t % S::kValueStages], t / S::kValueStages & 1, given_up, &g_status);
+                    if (fine) load_values(t + S::kValueStages);
+                }
+            }
+        }
+    } else if (warp == 4) {
         // The instructions are issued one after the other by one thread, whose own pace counts: descriptors are sums with
         // constants, loops are unrolled.
         constexpr bool bf16 = __is_same(T, __nv_bfloat16);
@@ -232,17 +259,17 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
                 for (int n = 0; n < DP / 16; ++n)
                     tc5::mma_f16(s_at, q_desc + ((n >> 2) * (kRows * 128 >> 4) + (n & 3) * 2), kd + ((n >> 2) * (kKeys * 128 >> 4) + (n & 3) * 2), idesc_s, n > 0);
                 tc5::commit(&s_full[t % S::kBuffers]);
+                if (S::kCopyWarp) tc5::commit(&k_free[t % S::kKeyStages]);
             }
         };
-        int sv = 0;  // the place of tile t's values, and its turn
-        uint32_t v_turn = 0;
         if (count > 0) {
             fine = tc5::wait_warp(q_ready, 0, given_up, &g_status);
             scores(0);
         }
         for (int t = 0; t < count && fine; ++t) {
             if (S::kBuffers == 2 && t + 1 < count) scores(t + 1);
-            fine = fine && tc5::wait_warp(&v_full[sv], v_turn, given_up, &g_status);
+            const int sv = t % S::kValueStages;
+            fine = fine && tc5::wait_warp(&v_full[sv], t / S::kValueStages & 1, given_up, &g_status);
             const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
             if (fine && (valid & 15)) {
                 // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
@@ -266,10 +293,16 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
                     for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, t > 0 || n > 0);
                 }
                 if (S::kBuffers == 2 || t + 1 == count) tc5::commit(&o_done[t % S::kBuffers]);
+                if (S::kCopyWarp) tc5::commit(&v_free[sv]);
             }
             __syncwarp();
             if (S::kBuffers == 1 && t + 1 < count) scores(t + 1);
-            if (++sv == S::kValueStages) sv = 0, v_turn ^= 1;
+            // Tile t + 1's S is on its way, or tile t's weights were there: tile t's keys and, before them, tile t - 1's values
+            // have been read.
+            if (!S::kCopyWarp && fine && tc5::elect()) {
+                if (t > 0 && t + 1 < count) load_values(t + 1);
+                if (t + S::kKeyStages < count) load_keys(t + S::kKeyStages);
+            }
         }
         if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
             tc5::commit(o_done);
@@ -309,54 +342,37 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
             fine = tc5::wait_warp(&s_full[buffer], t / S::kBuffers & 1, given_up, &g_status);
             if (!fine) break;
             tc5::after_sync();
-            if (threadIdx.x == 0) {  // the tiles that have been read make room for others
-                if (t + 1 < count) load_values(t + 1);
-                if (t + 2 < count) load_keys(t + 2);
-            }
-            __syncwarp();
             if (warp_there) {  // (else nothing but rows that are not there: their weights are whatever lies in the place)
                 const uint32_t s_at = tmem + lanes + buffer * kKeys;
                 const int j0 = base + t * kKeys;
-                float shift = -m * a.c;
-                const float2 c2 = {a.c, a.c};
-                float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-                uint32_t s[2][32], p[2][16];
-                // 32 weights, two at a time, and what else there is to do beside them
-                const auto weights = [&](int n, auto beside) {
-                    const float2 shift2 = {shift, shift};
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float2 z = fma2({__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1])}, c2, shift2);
-                        z.x = ex2(z.x);
-                        z.y = ex2(z.y);
-                        sum[e & 1] = add2(sum[e & 1], z);
-                        p[n][e] = pack<T>(z.x, z.y);
-                        beside(e);
-                    }
-                };
-                tc5::ld32(s[0], s_at);
-                tc5::ld32(s[1], s_at + 32);
-                tc5::ld_wait(s[0]);
-                tc5::ld_wait(s[1]);
                 // In a tile that every row sees all of, the weights are worked out with the maximum there was before, and
                 // the tile's own maximum beside them.  It hardly ever outgrows the other by as much as it may.
                 bool careful = t == 0 || last_lo > j0 || first_hi < j0 + kKeys;
                 if (!careful) {
+                    uint32_t s[2][32], p[2][16];
+                    tc5::ld64(s[0], s[1], s_at);
+                    const float shift = -m * a.c;
                     float top[2] = {-INFINITY, -INFINITY};
-                    weights(0, [&](int e) {
-                        top[0] = max3(top[0], __uint_as_float(s[0][e * 2]), __uint_as_float(s[0][e * 2 + 1]));
-                        top[1] = max3(top[1], __uint_as_float(s[1][e * 2]), __uint_as_float(s[1][e * 2 + 1]));
-                    });
-                    weights(1, [](int) {});
+                    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float u = __uint_as_float(s[n][e * 2]), w = __uint_as_float(s[n][e * 2 + 1]);
+                            top[e & 1] = max3(top[e & 1], u, w);
+                            p[n][e] = weights<T>(u, w, a.c, shift, sum[e & 1]);
+                        }
                     careful = __any_sync(0xffffffffu, !((fmaxf(top[0], top[1]) - m) * a.c <= kLazy));
-                    if (careful) {
-                        tc5::ld32(s[0], s_at);
-                        tc5::ld32(s[1], s_at + 32);
-                        tc5::ld_wait(s[0]);
-                        tc5::ld_wait(s[1]);
+                    if (!careful) {
+                        tc5::st16(s_at, p[0]);
+                        tc5::st16(s_at + 16, p[1]);
+                        sum[0] = add2(sum[0], sum[1]);
+                        l += sum[0].x + sum[0].y;
                     }
                 }
                 if (careful) {
+                    uint32_t s[2][32];
+                    tc5::ld64(s[0], s[1], s_at);
                     float most = -INFINITY;
                     bool none[2];
 #pragma unroll
@@ -392,28 +408,27 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
                         for (int n = 0; n < DP; n += 16) {
                             uint32_t o[16];
                             tc5::ld16(o, o_at + n);
-                            tc5::ld_wait(o);
 #pragma unroll
                             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
                             tc5::st16(o_at + n, o);
                         }
                     }
-                    shift = m == -INFINITY ? 0.f : -m * a.c;
-                    sum[0] = sum[1] = {0.f, 0.f};
+                    const float shift = m == -INFINITY ? 0.f : -m * a.c;
+                    float2 sum = {0.f, 0.f};
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
+                        uint32_t p[16];
                         if (none[n]) {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) p[n][e] = 0;
+                            for (int e = 0; e < 16; ++e) p[e] = 0;
                         } else {
-                            weights(n, [](int) {});
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) p[e] = weights<T>(__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1]), a.c, shift, sum);
                         }
+                        tc5::st16(s_at + n * 16, p);
                     }
+                    l += sum.x + sum.y;
                 }
-                tc5::st16(s_at, p[0]);
-                tc5::st16(s_at + 16, p[1]);
-                sum[0] = add2(sum[0], sum[1]);
-                l += sum[0].x + sum[0].y;
                 tc5::st_wait();
             }
             if (!fine) break;
@@ -441,7 +456,6 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kBlocks) attention_kernel
                 __syncwarp();
                 if (any) {
                     tc5::ld32(o, o_at + n);
-                    tc5::ld_wait(o);
                 }
                 if (!there) continue;
 #pragma unroll
@@ -555,7 +569,7 @@ int launch(const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStre
     const auto kernel = attention_kernel<T, DP>;
     if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kBytes))) return rc;
     const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
-    kernel<<<(unsigned)blocks, kThreads, Shape<DP>::kBytes, stream>>>(a, mk, mv);
+    kernel<<<(unsigned)blocks, Shape<DP>::kThreads, Shape<DP>::kBytes, stream>>>(a, mk, mv);
     if (const int rc = ofe::launched()) return rc;
     if (a.splits == 1) return OPENFISH_B200_OK;
     const long long joins = ((long long)a.max_q * a.q_heads * a.sequences + 3) / 4;

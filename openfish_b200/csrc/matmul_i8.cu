@@ -166,8 +166,6 @@ __global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const
             for (int c = 0; c < BN; c += 64, ++turn) {
                 const uint32_t sum = tmem + ((uint32_t)(quarter * 32) << 16) + (j & 1) * BN + c;
                 uint32_t v[2][32];
-                tc5::ld32(v[0], sum);
-                tc5::ld32(v[1], sum + 32);
                 __syncwarp();
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -181,8 +179,7 @@ __global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const
                 }
                 if (lane == 0) tc5::store_wait_read<1>();  // the copy out of this half of the staging memory is done with it
                 __syncwarp();
-                tc5::ld_wait(v[0]);
-                tc5::ld_wait(v[1]);
+                tc5::ld64(v[0], v[1], sum);
                 if (c + 64 >= BN) {  // the accumulator has been read: the next tile's sums may go there
                     tc5::before_sync();
                     if (lane == 0) {
