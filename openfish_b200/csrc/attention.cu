@@ -4,17 +4,20 @@
 //
 // in one pass over the keys: m_i is a running maximum, and what has been summed is scaled when it moves.
 //
-// A block takes 128 rows of one sequence and key head against the keys in tiles of 64; several blocks share an SM.  The
-// query heads that share a key head are rows next to each other (row r is query r / g, head r % g of the group), so
-// that grouped heads and single tokens fill the same tiles and a key is read once for all of them.
+// A block takes the rows of one sequence and key head, 128 or two halves of 128, against the keys in tiles of 64.  The query
+// heads that share a key head are rows next to each other (row r is query r / g, head r % g of the group), so that
+// grouped heads and single tokens fill the same tiles and a key is read once for all of them.
 //
-//   warps 0-3  the softmax, a thread to a row
-//   warp 4     the matrix instructions, S = Q K^T into tensor memory and O += P V with P read from there, in S's place; and the
-//              asynchronous copies of the keys' and values' tiles
+//   4 warps to a half   the softmax, a thread to a row
+//   1 warp to a half    the matrix instructions: S = Q K^T into tensor memory, O += P V with P read from there, in S's place
+//   1 warp              asynchronous copies of the keys' and values' tiles (heads of up to 64: the last warp above)
 //
-// Tensor memory and registers decide how many blocks there are to an SM, and only other blocks' work fills the waits between a
-// tile's steps.  Heads of up to 64: S and O take 128 columns, four blocks.  Heads of up to 128: O alone takes that, so two
-// blocks, each with two S in turn: the next tile's S is formed while this tile's weights are worked out.
+// Tensor memory and registers decide how many halves there are to an SM, and only other halves' work fills the waits between a
+// tile's steps.  Heads of up to 64: S and O take 128 columns, four blocks of a half.  Heads of up to 128: O alone takes
+// that, so two halves, each with two S in turn: the next tile's S is formed while this tile's weights are worked out.  The
+// two share a block and its tiles, for the copies' way into shared memory and the products' way out of it are what bounds
+// these heads: 48 cycles for each 128 x 64 x 16 of Q K^T (6 KB), 64 for 128 x 128 x 16 of P V.  Where there are rows for one half only (single
+// tokens), a block has one, and an SM two blocks.
 #include <math.h>
 #include <stdint.h>
 
@@ -25,7 +28,7 @@ namespace {
 
 __device__ int g_status;  // of the kernels on this device: a wait that ran out
 
-constexpr int kRows = 128;  // of a block
+constexpr int kRows = 128;  // of a half
 constexpr int kKeys = 64;   // of a tile
 constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled: weights up to 256
 
@@ -106,17 +109,18 @@ __device__ __forceinline__ uint32_t weights(float u, float w, float c, float shi
     return pack<T>(z.x, z.y);
 }
 
-template <int DP>
+template <int DP, int H>
 struct Shape {
-    static constexpr int kBuffers = DP == 64 ? 1 : 2, kBlocks = DP == 64 ? 4 : 2;  // S at a time; blocks to an SM
-    static constexpr int kChunks = DP / 64;                                        // of 64 elements, 128 bytes
+    static constexpr int kBuffers = DP == 64 ? 1 : 2;           // S at a time
+    static constexpr int kBlocks = (DP == 64 ? 4 : 2) / H;      // to an SM
+    static constexpr int kChunks = DP / 64;                     // of 64 elements, 128 bytes
     static constexpr int kQueryBytes = kChunks * kRows * 128, kTileBytes = kChunks * kKeys * 128;
-    static constexpr int kKeyStages = kBuffers + 1, kValueStages = 2;
-    // a warp of its own starts the copies where registers allow one
-    static constexpr bool kCopyWarp = DP == 128;
-    static constexpr int kThreads = kCopyWarp ? 192 : 160;
-    static constexpr int kBytes = kQueryBytes + (kKeyStages + kValueStages) * kTileBytes + (2 * (kKeyStages + kValueStages) + 3 * kBuffers + 1) * 8 + 8;
-    static constexpr int kColumns = kBuffers * kKeys + DP, kOut = kBuffers * kKeys;  // of tensor memory, a power of two; O's first
+    static constexpr int kKeyStages = DP == 64 ? 2 : 3 * H, kValueStages = 2 * H;
+    static constexpr bool kCopyWarp = DP == 128;                // a warp of its own for the copies, where registers allow one
+    static constexpr int kThreads = 32 * (5 * H + kCopyWarp);
+    static constexpr int kBytes = H * kQueryBytes + (kKeyStages + kValueStages) * kTileBytes + (2 * (kKeyStages + kValueStages) + H * (3 * kBuffers + 1)) * 8 + 8;
+    // columns of tensor memory, a power of two: S and O of each half
+    static constexpr int kHalfColumns = kBuffers * kKeys + DP, kColumns = H * kHalfColumns, kOut = kBuffers * kKeys;
 };
 
 // One row again, by a warp, straight from its definition and reading only the keys that the row sees.  A matrix
@@ -159,10 +163,10 @@ __device__ __noinline__ float2 redo_row(const T *q, const T *k, const T *v, long
     return make_float2(m, l);
 }
 
-template <class T, int DP>
-__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
-                                                                                 const __grid_constant__ CUtensorMap map_v) {
-    using S = Shape<DP>;
+template <class T, int DP, int H>
+__global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
+                                                                                                  const __grid_constant__ CUtensorMap map_v) {
+    using S = Shape<DP, H>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- which rows, which keys.  The last rows come first: under a causal mask they have the most keys.
@@ -172,22 +176,37 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
     int q0, nq, k0, nk;
     span(a.q_start, a.q_used, seq, a.q_rows, a.max_q, &q0, &nq);
     span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
-    const int rows = nq * a.group, r0 = block * kRows;
+    const int rows = nq * a.group, r0 = block * H * kRows;
     if (r0 >= rows) return;
-    int lo, hi, unused;  // the keys that the rows see between them
-    window(a, by_group(a, r0), nq, nk, &lo, &unused);
-    window(a, by_group(a, min(r0 + kRows, rows) - 1), nq, nk, &unused, &hi);
-    const int tiles = (max(hi - lo, 0) + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
+    int lo[H], hi[H];  // the keys that a half's rows see between them
+    int all_lo = 0, all_hi = 0;
+#pragma unroll
+    for (int x = 0; x < H; ++x) {
+        int unused;
+        lo[x] = hi[x] = 0;
+        if (r0 + x * kRows >= rows) continue;
+        window(a, by_group(a, r0 + x * kRows), nq, nk, &lo[x], &unused);
+        window(a, by_group(a, min(r0 + (x + 1) * kRows, rows) - 1), nq, nk, &unused, &hi[x]);
+        if (hi[x] <= lo[x]) continue;
+        all_lo = all_hi == 0 ? lo[x] : min(all_lo, lo[x]);
+        all_hi = max(all_hi, hi[x]);
+    }
+    const int tiles = (all_hi - all_lo + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
     const int first = min(split * per, tiles), count = min(per, tiles - first);  // this split's tiles
-    const int base = lo + first * kKeys;                                         // and its first key
+    const int base = all_lo + first * kKeys;                                     // and its first key
+    int from[H], to[H];                                                          // each half's of them
+#pragma unroll
+    for (int x = 0; x < H; ++x) {
+        from[x] = max((lo[x] - base) / kKeys, 0);  // (a negative difference rounds up: no further than 0)
+        to[x] = hi[x] <= lo[x] ? 0 : min(max(hi[x] - base + kKeys - 1, 0) / kKeys, count);
+        if (to[x] <= from[x]) from[x] = to[x] = 0;
+    }
 
-    extern __shared__ __align__(1024) uint8_t q_tile[];  // the swizzle counts from 1024-byte boundaries
-    uint8_t *const k_tiles = q_tile + S::kQueryBytes, *const v_tiles = k_tiles + S::kKeyStages * S::kTileBytes;
+    extern __shared__ __align__(1024) uint8_t q_tiles[];  // the swizzle counts from 1024-byte boundaries
+    uint8_t *const k_tiles = q_tiles + H * S::kQueryBytes, *const v_tiles = k_tiles + S::kKeyStages * S::kTileBytes;
     uint64_t *const k_full = reinterpret_cast<uint64_t *>(v_tiles + S::kValueStages * S::kTileBytes), *const v_full = k_full + S::kKeyStages;
-    uint64_t *const k_free = v_full + S::kValueStages, *const v_free = k_free + S::kKeyStages;
-    uint64_t *const s_full = v_free + S::kValueStages, *const p_ready = s_full + S::kBuffers, *const q_ready = p_ready + S::kBuffers;
-    uint64_t *const o_done = q_ready + 1;
-    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(o_done + S::kBuffers);
+    uint64_t *const k_free = v_full + S::kValueStages, *const v_free = k_free + S::kKeyStages, *const of_half = v_free + S::kValueStages;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(of_half + H * (3 * S::kBuffers + 1));
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const auto load_keys = [&](int t) {
@@ -206,13 +225,14 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
     };
     if (threadIdx.x == 0) {
         *given_up = 0;
-        for (int i = 0; i < 2 * (S::kKeyStages + S::kValueStages); ++i) ofd::mbar_init(&k_full[i], 1);
-        for (int i = 0; i < S::kBuffers; ++i) {
-            ofd::mbar_init(&s_full[i], 1);
-            ofd::mbar_init(&p_ready[i], 4);
-            ofd::mbar_init(&o_done[i], 1);
+        for (int i = 0; i < S::kKeyStages + S::kValueStages; ++i) {
+            ofd::mbar_init(&k_full[i], 1);
+            ofd::mbar_init(&k_free[i], H);
         }
-        ofd::mbar_init(q_ready, 4);
+        for (int i = 0; i < H * (3 * S::kBuffers + 1); ++i) {
+            // of each half: s_full and o_done (a commit each), p_ready and q_ready (an arrival of each warp)
+            ofd::mbar_init(&of_half[i], i % (3 * S::kBuffers + 1) < 2 * S::kBuffers ? 1 : 4);
+        }
         ofd::mbar_fence_init();
         if (count > 0) {
             load_keys(0);
@@ -221,13 +241,17 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
             for (int t = 1; t < S::kValueStages && t < count; ++t) load_values(t);
         }
     }
-    if (warp == 4) tc5::tmem_alloc<1>(tmem_slot, S::kColumns);
+    if (warp == 4 * H) tc5::tmem_alloc<1>(tmem_slot, S::kColumns);
     tc5::before_sync();
     __syncthreads();
     tc5::after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const int x = warp < 4 * H ? warp >> 2 : warp - 4 * H;  // this warp's half
+    uint64_t *const s_full = of_half + x * (3 * S::kBuffers + 1), *const o_done = s_full + S::kBuffers, *const p_ready = o_done + S::kBuffers;
+    uint64_t *const q_ready = p_ready + S::kBuffers;
+    const uint32_t tmem = *tmem_slot + x * S::kHalfColumns;
+    uint8_t *const q_tile = q_tiles + x * S::kQueryBytes;
 
-    if (S::kCopyWarp && warp == 5) {
+    if (warp == 5 * H) {
         if (lane == 0) {
             bool fine = true;
             for (int t = 0; t < count && fine; ++t) {
@@ -241,60 +265,66 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
                 }
             }
         }
-    } else if (warp == 4) {
+    } else if (warp >= 4 * H) {
         // The instructions are issued one after the other by one thread, whose own pace counts: descriptors are sums with
         // constants, loops are unrolled.
         constexpr bool bf16 = __is_same(T, __nv_bfloat16);
         constexpr uint32_t idesc_s = tc5::idesc_f16(128, kKeys, bf16, false), idesc_o = tc5::idesc_f16(128, DP, bf16, true);
         const uint64_t q_desc = tc5::desc_k_major(tc5::smem_u32(q_tile)), k_desc = tc5::desc_k_major(tc5::smem_u32(k_tiles));
         const uint64_t v_desc = tc5::desc_mn_major(tc5::smem_u32(v_tiles), kKeys * 128);
+        const int begin = H == 1 ? 0 : from[x], end = H == 1 ? count : to[x];
         bool fine = true;
         const auto scores = [&](int t) {  // S = Q K^T of tile t
-            fine = fine && tc5::wait_warp(&k_full[t % S::kKeyStages], t / S::kKeyStages & 1, given_up, &g_status);
+            const int sk = t % S::kKeyStages, u = t - begin;
+            fine = fine && tc5::wait_warp(&k_full[sk], t / S::kKeyStages & 1, given_up, &g_status);
             tc5::after_sync();
-            const uint32_t s_at = tmem + t % S::kBuffers * kKeys;
-            const uint64_t kd = k_desc + (uint32_t)(t % S::kKeyStages * (S::kTileBytes >> 4));
+            const uint32_t s_at = tmem + u % S::kBuffers * kKeys;
+            const uint64_t kd = k_desc + (uint32_t)(sk * (S::kTileBytes >> 4));
             if (fine && tc5::elect()) {
+                if (H == 1 || (t >= begin && t < end)) {
 #pragma unroll
-                for (int n = 0; n < DP / 16; ++n)
-                    tc5::mma_f16(s_at, q_desc + ((n >> 2) * (kRows * 128 >> 4) + (n & 3) * 2), kd + ((n >> 2) * (kKeys * 128 >> 4) + (n & 3) * 2), idesc_s, n > 0);
-                tc5::commit(&s_full[t % S::kBuffers]);
-                if (S::kCopyWarp) tc5::commit(&k_free[t % S::kKeyStages]);
+                    for (int n = 0; n < DP / 16; ++n)
+                        tc5::mma_f16(s_at, q_desc + ((n >> 2) * (kRows * 128 >> 4) + (n & 3) * 2), kd + ((n >> 2) * (kKeys * 128 >> 4) + (n & 3) * 2), idesc_s, n > 0);
+                    tc5::commit(&s_full[u % S::kBuffers]);
+                }
+                if (S::kCopyWarp) tc5::commit(&k_free[sk]);
             }
         };
         if (count > 0) {
-            fine = tc5::wait_warp(q_ready, 0, given_up, &g_status);
+            if (end > begin) fine = tc5::wait_warp(q_ready, 0, given_up, &g_status);
             scores(0);
         }
         for (int t = 0; t < count && fine; ++t) {
             if (S::kBuffers == 2 && t + 1 < count) scores(t + 1);
-            const int sv = t % S::kValueStages;
+            const int sv = t % S::kValueStages, u = t - begin;
             fine = fine && tc5::wait_warp(&v_full[sv], t / S::kValueStages & 1, given_up, &g_status);
-            const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
-            if (fine && (valid & 15)) {
-                // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
-                const int behind = 16 - (valid & 15);
-                for (int n = lane; n < behind * 8 * S::kChunks; n += 32) {
-                    const int d = n / (behind * 8), in = n % (behind * 8);
-                    *reinterpret_cast<uint4 *>(v_tiles + sv * S::kTileBytes + d * kKeys * 128 + valid * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+            if (H == 1 || (t >= begin && t < end)) {
+                const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
+                if (fine && (valid & 15)) {
+                    // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
+                    const int behind = 16 - (valid & 15);
+                    for (int n = lane; n < behind * 8 * S::kChunks; n += 32) {
+                        const int d = n / (behind * 8), in = n % (behind * 8);
+                        *reinterpret_cast<uint4 *>(v_tiles + sv * S::kTileBytes + d * kKeys * 128 + valid * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    tc5::fence_async();
+                    __syncwarp();
                 }
-                tc5::fence_async();
-                __syncwarp();
-            }
-            const uint64_t vd = v_desc + (uint32_t)(sv * (S::kTileBytes >> 4));
-            const uint32_t o_at = tmem + S::kOut, p_at = tmem + t % S::kBuffers * kKeys;
-            fine = fine && tc5::wait_warp(&p_ready[t % S::kBuffers], t / S::kBuffers & 1, given_up, &g_status);
-            tc5::after_sync();
-            if (fine && tc5::elect()) {
-                if (steps == 4) {
+                const uint64_t vd = v_desc + (uint32_t)(sv * (S::kTileBytes >> 4));
+                const uint32_t o_at = tmem + S::kOut, p_at = tmem + u % S::kBuffers * kKeys;
+                fine = fine && tc5::wait_warp(&p_ready[u % S::kBuffers], u / S::kBuffers & 1, given_up, &g_status);
+                tc5::after_sync();
+                if (fine && tc5::elect()) {
+                    if (steps == 4) {
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, t > 0 || n > 0);
-                } else {
-                    for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, t > 0 || n > 0);
+                        for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, u > 0 || n > 0);
+                    } else {
+                        for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, u > 0 || n > 0);
+                    }
+                    if (S::kBuffers == 2 || t + 1 == end) tc5::commit(&o_done[u % S::kBuffers]);
                 }
-                if (S::kBuffers == 2 || t + 1 == count) tc5::commit(&o_done[t % S::kBuffers]);
-                if (S::kCopyWarp) tc5::commit(&v_free[sv]);
             }
+            if (S::kCopyWarp && fine && tc5::elect()) tc5::commit(&v_free[sv]);
             __syncwarp();
             if (S::kBuffers == 1 && t + 1 < count) scores(t + 1);
             // Tile t + 1's S is on its way, or tile t's weights were there: tile t's keys and, before them, tile t - 1's values
@@ -309,15 +339,16 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
             ofd::mbar_land(o_done, 0, 0, ofd::kDefaultWaitLimitNs);
         }
     } else {
-        const int row = warp * 32 + lane;  // of the block, and lane of tensor memory
-        const int r = r0 + row, i = by_group(a, r), head = kh * a.group + r - i * a.group;
-        const bool there = r < rows, warp_there = r0 + warp * 32 < rows;
+        const int begin = H == 1 ? 0 : from[x], end = H == 1 ? count : to[x];
+        const int row = (warp & 3) * 32 + lane, half0 = r0 + x * kRows;  // of the half, and lane of tensor memory; the half's first
+        const int r = half0 + row, i = by_group(a, r), head = kh * a.group + r - i * a.group;
+        const bool there = r < rows, warp_there = half0 + (warp & 3) * 32 < rows;
         // ---- the queries into shared memory, pieces of 16 bytes; zeros where there are none
-        if (count > 0) {
+        if (end > begin) {
             constexpr int kPieces = DP / 8;
 #pragma unroll 4
-            for (int n = threadIdx.x; n < kRows * kPieces; n += 128) {
-                const int qr = n / kPieces, p = n % kPieces, rr = r0 + qr, ri = by_group(a, rr);
+            for (int n = threadIdx.x & 127; n < kRows * kPieces; n += 128) {
+                const int qr = n / kPieces, p = n % kPieces, rr = half0 + qr, ri = by_group(a, rr);
                 uint4 val = make_uint4(0, 0, 0, 0);
                 if (rr < rows && p * 8 < a.head_dim)
                     val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(q0 + ri) * a.q_stride_row +
@@ -335,11 +366,11 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
         const int first_lo = __shfl_sync(0xffffffffu, my_lo, 0), first_hi = __shfl_sync(0xffffffffu, my_hi, 0);
         const int last_lo = __shfl_sync(0xffffffffu, my_lo, 31), last_hi = __shfl_sync(0xffffffffu, my_hi, 31);
         float m = -INFINITY, l = 0.f;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16, o_at = tmem + lanes + S::kOut;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lanes + S::kOut;
         bool fine = true;
-        for (int t = 0; t < count; ++t) {
-            const int buffer = t % S::kBuffers;
-            fine = tc5::wait_warp(&s_full[buffer], t / S::kBuffers & 1, given_up, &g_status);
+        for (int t = begin; t < end; ++t) {
+            const int u = t - begin, buffer = u % S::kBuffers;
+            fine = tc5::wait_warp(&s_full[buffer], u / S::kBuffers & 1, given_up, &g_status);
             if (!fine) break;
             tc5::after_sync();
             if (warp_there) {  // (else nothing but rows that are not there: their weights are whatever lies in the place)
@@ -347,7 +378,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
                 const int j0 = base + t * kKeys;
                 // In a tile that every row sees all of, the weights are worked out with the maximum there was before, and
                 // the tile's own maximum beside them.  It hardly ever outgrows the other by as much as it may.
-                bool careful = t == 0 || last_lo > j0 || first_hi < j0 + kKeys;
+                bool careful = u == 0 || last_lo > j0 || first_hi < j0 + kKeys;
                 if (!careful) {
                     uint32_t s[2][32], p[2][16];
                     tc5::ld64(s[0], s[1], s_at);
@@ -401,7 +432,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
                     }
                     if (__any_sync(0xffffffffu, fade != 1.f)) {
                         // the sums so far: with one S they are there when it is
-                        if (S::kBuffers == 2) fine = tc5::wait_warp(&o_done[buffer ^ 1], (t - 1) / 2 & 1, given_up, &g_status);
+                        if (S::kBuffers == 2) fine = tc5::wait_warp(&o_done[buffer ^ 1], (u - 1) / 2 & 1, given_up, &g_status);
                         tc5::after_sync();
                         l *= fade;
 #pragma unroll 1
@@ -437,9 +468,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
             if (lane == 0) tc5::arrive(&p_ready[buffer]);
         }
         // ---- out = O / l
-        const bool any = fine && count > 0;
+        const bool any = fine && end > begin;
         if (any) {
-            fine = tc5::wait_warp(&o_done[(count - 1) % S::kBuffers], S::kBuffers == 2 ? (count - 1) / 2 & 1 : 0, given_up, &g_status);
+            const int last = end - begin - 1;
+            fine = tc5::wait_warp(&o_done[last % S::kBuffers], S::kBuffers == 2 ? last / 2 & 1 : 0, given_up, &g_status);
             tc5::after_sync();
         }
         if (fine && warp_there) {
@@ -479,7 +511,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
             __syncwarp();
             for (uint32_t again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
                 const int who = __ffs(again) - 1;
-                const int rr = r0 + warp * 32 + who, ii = by_group(a, rr), hh = kh * a.group + rr - ii * a.group;
+                const int rr = half0 + (warp & 3) * 32 + who, ii = by_group(a, rr), hh = kh * a.group + rr - ii * a.group;
                 const int klo = __shfl_sync(0xffffffffu, in_lo, who), khi = __shfl_sync(0xffffffffu, in_hi, who);
                 const long long aa = (long long)(q0 + ii) * a.q_heads + hh;
                 const float2 ml = redo_row<T>(static_cast<const T *>(a.q) + (long long)(q0 + ii) * a.q_stride_row + hh * a.q_stride_head,
@@ -503,7 +535,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kBlocks) atten
             ofd::mbar_land(&k_full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
         }
     }
-    if (warp == 4) tc5::tmem_free<1>(tmem, S::kColumns);
+    if (warp == 4 * H) tc5::tmem_free<1>(tmem, S::kColumns);
 }
 
 // The splits' results joined: out = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A warp to a query and head.
@@ -540,14 +572,17 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
     }
 }
 
+// Halves to a block.
+int halves_for(const openfish_b200_attention_t *a) { return a->head_dim > 64 && (long long)a->max_q * (a->q_heads / a->kv_heads) > kRows ? 2 : 1; }
+
 // Into how many pieces a block's keys go: enough blocks to fill the SMs, four tiles of keys to a piece at least.
 int splits_for(const openfish_b200_attention_t *a, int sms) {
-    const long long group = a->q_heads / a->kv_heads;
-    const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64>::kBlocks : Shape<128>::kBlocks);
-    const long long blocks = (a->max_q * group + kRows - 1) / kRows * a->kv_heads * a->sequences;
+    const long long group = a->q_heads / a->kv_heads, halves = halves_for(a), rows = halves * kRows;
+    const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64, 1>::kBlocks : Shape<128, 1>::kBlocks / halves);
+    const long long blocks = (a->max_q * group + rows - 1) / rows * a->kv_heads * a->sequences;
     long long keys = a->max_k;
     if (a->window_left >= 0 && a->window_right >= 0) {
-        const long long seen = (long long)a->window_left + a->window_right + 1 + kRows / group;
+        const long long seen = (long long)a->window_left + a->window_right + 1 + rows / group;
         if (seen < keys) keys = seen;
     }
     const long long tiles = (keys + kKeys - 1) / kKeys;
@@ -564,17 +599,24 @@ bool heads_map(CUtensorMap *map, bool bf16, const void *base, const openfish_b20
     return tc5::make_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box);
 }
 
-template <class T, int DP>
+template <class T, int DP, int H>
 int launch(const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
-    const auto kernel = attention_kernel<T, DP>;
-    if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kBytes))) return rc;
+    using S = Shape<DP, H>;
+    const auto kernel = attention_kernel<T, DP, H>;
+    if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
     const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
-    kernel<<<(unsigned)blocks, Shape<DP>::kThreads, Shape<DP>::kBytes, stream>>>(a, mk, mv);
+    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mk, mv);
     if (const int rc = ofe::launched()) return rc;
     if (a.splits == 1) return OPENFISH_B200_OK;
     const long long joins = ((long long)a.max_q * a.q_heads * a.sequences + 3) / 4;
     attention_join_kernel<T><<<(unsigned)(joins < 16384 ? joins : 16384), 128, 0, stream>>>(a);
     return ofe::launched();
+}
+
+template <class T>
+int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, int halves, cudaStream_t stream) {
+    if (p->head_dim <= 64) return launch<T, 64, 1>(a, mk, mv, stream);
+    return halves == 1 ? launch<T, 128, 1>(a, mk, mv, stream) : launch<T, 128, 2>(a, mk, mv, stream);
 }
 
 size_t part_bytes(const openfish_b200_attention_t *a, int splits) {
@@ -610,7 +652,8 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     a.group_shift = (uint32_t)bits;
     a.group_mul = (uint32_t)(((1ull << 32) * ((1ull << bits) - (unsigned)a.group)) / (unsigned)a.group + 1);
     a.c = p->scale * 1.4426950408889634f;
-    a.tiles = (int)(((long long)p->max_q * a.group + kRows - 1) / kRows);
+    const int halves = halves_for(p);
+    a.tiles = (int)(((long long)p->max_q * a.group + halves * kRows - 1) / (halves * kRows));
     a.splits = splits_for(p, sms);
     a.part_lse = static_cast<float *>(p->workspace);
     a.part = a.part_lse;
@@ -629,8 +672,7 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     }
     if (!heads_map(&mk, bf16, k, &none, p->k_stride_row, p->k_stride_head) || !heads_map(&mv, bf16, v, &none, p->v_stride_row, p->v_stride_head))
         return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
-    if (p->head_dim <= 64) return bf16 ? launch<__nv_bfloat16, 64>(a, mk, mv, (cudaStream_t)stream) : launch<__half, 64>(a, mk, mv, (cudaStream_t)stream);
-    return bf16 ? launch<__nv_bfloat16, 128>(a, mk, mv, (cudaStream_t)stream) : launch<__half, 128>(a, mk, mv, (cudaStream_t)stream);
+    return bf16 ? launch_for<__nv_bfloat16>(p, a, mk, mv, halves, (cudaStream_t)stream) : launch_for<__half>(p, a, mk, mv, halves, (cudaStream_t)stream);
 }
 
 extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }
