@@ -115,10 +115,13 @@ struct Shape {
     static constexpr int kBlocks = (DP == 64 ? 4 : 2) / H;      // to an SM
     static constexpr int kChunks = DP / 64;                     // of 64 elements, 128 bytes
     static constexpr int kQueryBytes = kChunks * kRows * 128, kTileBytes = kChunks * kKeys * 128;
-    static constexpr int kKeyStages = DP == 64 ? 2 : 3 * H, kValueStages = 2 * H;
+    // The ring moves in steps: step i brings the keys of tile i and the values of tile i - kBuffers, whose weights have the
+    // place that tile i's S goes to.
+    static constexpr int kStages = H == 2 ? 5 : 2, kStageBytes = 2 * kTileBytes;
     static constexpr bool kCopyWarp = DP == 128;                // a warp of its own for the copies, where registers allow one
     static constexpr int kThreads = 32 * (5 * H + kCopyWarp);
-    static constexpr int kBytes = H * kQueryBytes + (kKeyStages + kValueStages) * kTileBytes + (2 * (kKeyStages + kValueStages) + H * (3 * kBuffers + 1)) * 8 + 8;
+    static constexpr int kHalfBarriers = 2 * kBuffers + 3;      // s_full and p_ready of each S, q_ready, the last two o_done
+    static constexpr int kBytes = H * kQueryBytes + kStages * kStageBytes + (2 * kStages + H * kHalfBarriers) * 8 + 8;
     // columns of tensor memory, a power of two: S and O of each half
     static constexpr int kHalfColumns = kBuffers * kKeys + DP, kColumns = H * kHalfColumns, kOut = kBuffers * kKeys;
 };
@@ -203,136 +206,116 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     }
 
     extern __shared__ __align__(1024) uint8_t q_tiles[];  // the swizzle counts from 1024-byte boundaries
-    uint8_t *const k_tiles = q_tiles + H * S::kQueryBytes, *const v_tiles = k_tiles + S::kKeyStages * S::kTileBytes;
-    uint64_t *const k_full = reinterpret_cast<uint64_t *>(v_tiles + S::kValueStages * S::kTileBytes), *const v_full = k_full + S::kKeyStages;
-    uint64_t *const k_free = v_full + S::kValueStages, *const v_free = k_free + S::kKeyStages, *const of_half = v_free + S::kValueStages;
-    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(of_half + H * (3 * S::kBuffers + 1));
+    uint8_t *const ring = q_tiles + H * S::kQueryBytes;
+    uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kStageBytes), *const empty = full + S::kStages;
+    uint64_t *const of_half = empty + S::kStages;
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(of_half + H * S::kHalfBarriers);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const auto load_keys = [&](int t) {
-        uint64_t *const bar = &k_full[t % S::kKeyStages];
-        ofd::mbar_arrive_expect_tx(bar, S::kTileBytes);
+    const auto load = [&](int step, int stage) {
+        const bool keys = step < count, values = step >= S::kBuffers;
+        uint8_t *const at = ring + stage * S::kStageBytes;
+        ofd::mbar_arrive_expect_tx(&full[stage], ((int)keys + (int)values) * S::kTileBytes);
 #pragma unroll
-        for (int d = 0; d < S::kChunks; ++d)
-            tc5::load_3d(k_tiles + t % S::kKeyStages * S::kTileBytes + d * kKeys * 128, &map_k, d * 64, kh, k0 + base + t * kKeys, bar);
+        for (int d = 0; d < S::kChunks; ++d) {
+            if (keys) tc5::load_3d(at + d * kKeys * 128, &map_k, d * 64, kh, k0 + base + step * kKeys, &full[stage]);
+            if (values) tc5::load_3d(at + S::kTileBytes + d * kKeys * 128, &map_v, d * 64, kh, k0 + base + (step - S::kBuffers) * kKeys, &full[stage]);
+        }
     };
-    const auto load_values = [&](int t) {
-        uint64_t *const bar = &v_full[t % S::kValueStages];
-        ofd::mbar_arrive_expect_tx(bar, S::kTileBytes);
-#pragma unroll
-        for (int d = 0; d < S::kChunks; ++d)
-            tc5::load_3d(v_tiles + t % S::kValueStages * S::kTileBytes + d * kKeys * 128, &map_v, d * 64, kh, k0 + base + t * kKeys, bar);
-    };
+    const int steps = count > 0 ? count + S::kBuffers : 0;
     if (threadIdx.x == 0) {
         *given_up = 0;
-        for (int i = 0; i < S::kKeyStages + S::kValueStages; ++i) {
-            ofd::mbar_init(&k_full[i], 1);
-            ofd::mbar_init(&k_free[i], H);
+        for (int i = 0; i < S::kStages; ++i) {
+            ofd::mbar_init(&full[i], 1);
+            ofd::mbar_init(&empty[i], H);
         }
-        for (int i = 0; i < H * (3 * S::kBuffers + 1); ++i) {
-            // of each half: s_full and o_done (a commit each), p_ready and q_ready (an arrival of each warp)
-            ofd::mbar_init(&of_half[i], i % (3 * S::kBuffers + 1) < 2 * S::kBuffers ? 1 : 4);
+        for (int i = 0; i < H * S::kHalfBarriers; ++i) {
+            // s_full and o_done are a commit's, p_ready and q_ready take an arrival of each warp
+            const int of = i % S::kHalfBarriers;
+            ofd::mbar_init(&of_half[i], of < S::kBuffers || of > 2 * S::kBuffers ? 1 : 4);
         }
         ofd::mbar_fence_init();
-        if (count > 0) {
-            load_keys(0);
-            load_values(0);
-            for (int t = 1; t < S::kKeyStages && t < count; ++t) load_keys(t);
-            for (int t = 1; t < S::kValueStages && t < count; ++t) load_values(t);
-        }
+        for (int i = 0; i < S::kStages && i < steps; ++i) load(i, i);
     }
     if (warp == 4 * H) tc5::tmem_alloc<1>(tmem_slot, S::kColumns);
     tc5::before_sync();
     __syncthreads();
     tc5::after_sync();
     const int x = warp < 4 * H ? warp >> 2 : warp - 4 * H;  // this warp's half
-    uint64_t *const s_full = of_half + x * (3 * S::kBuffers + 1), *const o_done = s_full + S::kBuffers, *const p_ready = o_done + S::kBuffers;
-    uint64_t *const q_ready = p_ready + S::kBuffers;
+    uint64_t *const s_full = of_half + x * S::kHalfBarriers, *const p_ready = s_full + S::kBuffers, *const q_ready = p_ready + S::kBuffers;
+    uint64_t *const o_done = q_ready + 1;
     const uint32_t tmem = *tmem_slot + x * S::kHalfColumns;
     uint8_t *const q_tile = q_tiles + x * S::kQueryBytes;
 
     if (warp == 5 * H) {
         if (lane == 0) {
-            bool fine = true;
-            for (int t = 0; t < count && fine; ++t) {
-                if (t + S::kKeyStages < count) {
-                    fine = tc5::wait(&k_free[t % S::kKeyStages], t / S::kKeyStages & 1, given_up, &g_status);
-                    if (fine) load_keys(t + S::kKeyStages);
-                }
-                if (fine && t + S::kValueStages < count) {
-                    fine = tc5::wait(&v_free[t % S::kValueStages], t / S::kValueStages & 1, given_up, &g_status);
-                    if (fine) load_values(t + S::kValueStages);
-                }
+            int stage = 0;
+            uint32_t turn = 0;
+            for (int step = S::kStages; step < steps; ++step) {
+                if (!tc5::wait(&empty[stage], turn, given_up, &g_status)) break;
+                load(step, stage);
+                if (++stage == S::kStages) stage = 0, turn ^= 1;
             }
         }
     } else if (warp >= 4 * H) {
         // The instructions are issued one after the other by one thread, whose own pace counts: descriptors are sums with
-        // constants, loops are unrolled.
+        // constants, loops are unrolled, and O += P V of one tile and S of the next are one run of instructions.
         constexpr bool bf16 = __is_same(T, __nv_bfloat16);
         constexpr uint32_t idesc_s = tc5::idesc_f16(128, kKeys, bf16, false), idesc_o = tc5::idesc_f16(128, DP, bf16, true);
-        const uint64_t q_desc = tc5::desc_k_major(tc5::smem_u32(q_tile)), k_desc = tc5::desc_k_major(tc5::smem_u32(k_tiles));
-        const uint64_t v_desc = tc5::desc_mn_major(tc5::smem_u32(v_tiles), kKeys * 128);
+        const uint64_t q_desc = tc5::desc_k_major(tc5::smem_u32(q_tile));
         const int begin = H == 1 ? 0 : from[x], end = H == 1 ? count : to[x];
-        bool fine = true;
-        const auto scores = [&](int t) {  // S = Q K^T of tile t
-            const int sk = t % S::kKeyStages, u = t - begin;
-            fine = fine && tc5::wait_warp(&k_full[sk], t / S::kKeyStages & 1, given_up, &g_status);
-            tc5::after_sync();
-            const uint32_t s_at = tmem + u % S::kBuffers * kKeys;
-            const uint64_t kd = k_desc + (uint32_t)(sk * (S::kTileBytes >> 4));
-            if (fine && tc5::elect()) {
-                if (H == 1 || (t >= begin && t < end)) {
-#pragma unroll
-                    for (int n = 0; n < DP / 16; ++n)
-                        tc5::mma_f16(s_at, q_desc + ((n >> 2) * (kRows * 128 >> 4) + (n & 3) * 2), kd + ((n >> 2) * (kKeys * 128 >> 4) + (n & 3) * 2), idesc_s, n > 0);
-                    tc5::commit(&s_full[u % S::kBuffers]);
-                }
-                if (S::kCopyWarp) tc5::commit(&k_free[sk]);
-            }
-        };
-        if (count > 0) {
-            if (end > begin) fine = tc5::wait_warp(q_ready, 0, given_up, &g_status);
-            scores(0);
-        }
-        for (int t = 0; t < count && fine; ++t) {
-            if (S::kBuffers == 2 && t + 1 < count) scores(t + 1);
-            const int sv = t % S::kValueStages, u = t - begin;
-            fine = fine && tc5::wait_warp(&v_full[sv], t / S::kValueStages & 1, given_up, &g_status);
-            if (H == 1 || (t >= begin && t < end)) {
-                const int valid = min(nk - (base + t * kKeys), kKeys), steps = (valid + 15) / 16;  // of 16 keys
+        bool fine = end <= begin || tc5::wait_warp(q_ready, 0, given_up, &g_status);
+        int stage = 0;
+        uint32_t turn = 0;
+        for (int step = 0; step < steps && fine; ++step) {
+            // S of tile `step`, the half's tile `i`; O += P V of the one that had its place before
+            const int i = step - begin, buffer = i & (S::kBuffers - 1);
+            const bool scores = H == 1 ? step < count : step >= begin && step < end;
+            const bool sums = H == 1 ? step >= S::kBuffers : i >= S::kBuffers && step < end + S::kBuffers;
+            const uint32_t s_at = tmem + buffer * kKeys, o_at = tmem + S::kOut;
+            const uint64_t kd = tc5::desc_k_major(tc5::smem_u32(ring + stage * S::kStageBytes));
+            const uint64_t vd = tc5::desc_mn_major(tc5::smem_u32(ring + stage * S::kStageBytes + S::kTileBytes), kKeys * 128);
+            const int valid = min(nk - (base + (step - S::kBuffers) * kKeys), kKeys), pieces = (valid + 15) / 16;  // of 16 keys
+            fine = tc5::wait_warp(&full[stage], turn, given_up, &g_status);
+            if (sums) {
                 if (fine && (valid & 15)) {
-                    // rows behind the sequence's last key that the last step takes in: weights of zero, times what is there
+                    // rows behind the sequence's last key that the last piece takes in: weights of zero, times what is there
                     const int behind = 16 - (valid & 15);
                     for (int n = lane; n < behind * 8 * S::kChunks; n += 32) {
                         const int d = n / (behind * 8), in = n % (behind * 8);
-                        *reinterpret_cast<uint4 *>(v_tiles + sv * S::kTileBytes + d * kKeys * 128 + valid * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(ring + stage * S::kStageBytes + S::kTileBytes + d * kKeys * 128 + valid * 128 + in * 16) =
+                            make_uint4(0, 0, 0, 0);
                     }
                     tc5::fence_async();
                     __syncwarp();
                 }
-                const uint64_t vd = v_desc + (uint32_t)(sv * (S::kTileBytes >> 4));
-                const uint32_t o_at = tmem + S::kOut, p_at = tmem + u % S::kBuffers * kKeys;
-                fine = fine && tc5::wait_warp(&p_ready[u % S::kBuffers], u / S::kBuffers & 1, given_up, &g_status);
-                tc5::after_sync();
-                if (fine && tc5::elect()) {
-                    if (steps == 4) {
+                fine = fine && tc5::wait_warp(&p_ready[buffer], (i - S::kBuffers) / S::kBuffers & 1, given_up, &g_status);
+            }
+            tc5::after_sync();
+            if (fine && tc5::elect()) {
+                if (sums) {
+                    const bool more = i > S::kBuffers;
+                    if (pieces == 4) {
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, u > 0 || n > 0);
+                        for (int n = 0; n < 4; ++n) tc5::mma_f16_tmem(o_at, s_at + n * 8, vd + n * (2048 >> 4), idesc_o, more || n > 0);
                     } else {
-                        for (int n = 0; n < steps; ++n) tc5::mma_f16_tmem(o_at, p_at + n * 8, vd + n * (2048 >> 4), idesc_o, u > 0 || n > 0);
+                        for (int n = 0; n < pieces; ++n) tc5::mma_f16_tmem(o_at, s_at + n * 8, vd + n * (2048 >> 4), idesc_o, more || n > 0);
                     }
-                    if (S::kBuffers == 2 || t + 1 == end) tc5::commit(&o_done[u % S::kBuffers]);
                 }
+                if (scores) {
+#pragma unroll
+                    for (int n = 0; n < DP / 16; ++n)
+                        tc5::mma_f16(s_at, q_desc + ((n >> 2) * (kRows * 128 >> 4) + (n & 3) * 2), kd + ((n >> 2) * (kKeys * 128 >> 4) + (n & 3) * 2), idesc_s, n > 0);
+                    tc5::commit(&s_full[buffer]);
+                } else if (sums) {
+                    tc5::commit(&o_done[step - end]);  // the last ones, which no S follows
+                }
+                if (S::kCopyWarp) tc5::commit(&empty[stage]);
+                // The weights were there, so S before them was: the products of the last step are done.
+                else if (step > 0 && step + S::kStages - 1 < steps) load(step + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
             }
-            if (S::kCopyWarp && fine && tc5::elect()) tc5::commit(&v_free[sv]);
             __syncwarp();
-            if (S::kBuffers == 1 && t + 1 < count) scores(t + 1);
-            // Tile t + 1's S is on its way, or tile t's weights were there: tile t's keys and, before them, tile t - 1's values
-            // have been read.
-            if (!S::kCopyWarp && fine && tc5::elect()) {
-                if (t > 0 && t + 1 < count) load_values(t + 1);
-                if (t + S::kKeyStages < count) load_keys(t + S::kKeyStages);
-            }
+            if (++stage == S::kStages) stage = 0, turn ^= 1;
         }
         if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
             tc5::commit(o_done);
@@ -432,7 +415,9 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                     }
                     if (__any_sync(0xffffffffu, fade != 1.f)) {
                         // the sums so far: with one S they are there when it is
-                        if (S::kBuffers == 2) fine = tc5::wait_warp(&o_done[buffer ^ 1], (u - 1) / 2 & 1, given_up, &g_status);
+                        // (else they are when the next tile's S is, which is formed behind them)
+                        if (S::kBuffers == 2) fine = t + 1 < end ? tc5::wait_warp(&s_full[buffer ^ 1], (u + 1) / 2 & 1, given_up, &g_status)
+                                                                 : tc5::wait_warp(&o_done[0], 0, given_up, &g_status);
                         tc5::after_sync();
                         l *= fade;
 #pragma unroll 1
@@ -470,8 +455,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
         // ---- out = O / l
         const bool any = fine && end > begin;
         if (any) {
-            const int last = end - begin - 1;
-            fine = tc5::wait_warp(&o_done[last % S::kBuffers], S::kBuffers == 2 ? last / 2 & 1 : 0, given_up, &g_status);
+            fine = tc5::wait_warp(&o_done[S::kBuffers - 1], 0, given_up, &g_status);
             tc5::after_sync();
         }
         if (fine && warp_there) {
@@ -530,9 +514,9 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     __syncthreads();
     tc5::after_sync();
     if (*given_up && threadIdx.x == 0) {  // the copies under way land before the block ends
-        for (int n = 0; n < S::kKeyStages + S::kValueStages; ++n) {
-            uint64_t since = ofd::mbar_land(&k_full[n], 0, 0, ofd::kDefaultWaitLimitNs / 16);
-            ofd::mbar_land(&k_full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
+        for (int n = 0; n < S::kStages; ++n) {
+            const uint64_t since = ofd::mbar_land(&full[n], 0, 0, ofd::kDefaultWaitLimitNs / 16);
+            ofd::mbar_land(&full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
         }
     }
     if (warp == 4 * H) tc5::tmem_free<1>(tmem, S::kColumns);
