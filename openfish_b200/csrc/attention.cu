@@ -121,7 +121,7 @@ struct Shape {
     static constexpr bool kCopyWarp = DP == 128;                // a warp of its own for the copies, where registers allow one
     static constexpr int kThreads = 32 * (5 * H + kCopyWarp);
     static constexpr int kHalfBarriers = 2 * kBuffers + 3;      // s_full and p_ready of each S, q_ready, the last two o_done
-    static constexpr int kBytes = H * kQueryBytes + kStages * kStageBytes + (2 * kStages + H * kHalfBarriers) * 8 + 8;
+    static constexpr int kBytes = H * kQueryBytes + kStages * kStageBytes + (2 * kStages + H * (kHalfBarriers + 1)) * 8 + 8;
     // columns of tensor memory, a power of two: S and O of each half
     static constexpr int kHalfColumns = kBuffers * kKeys + DP, kColumns = H * kHalfColumns, kOut = kBuffers * kKeys;
 };
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     extern __shared__ __align__(1024) uint8_t q_tiles[];  // the swizzle counts from 1024-byte boundaries
     uint8_t *const ring = q_tiles + H * S::kQueryBytes;
     uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kStageBytes), *const empty = full + S::kStages;
-    uint64_t *const of_half = empty + S::kStages;
+    uint64_t *const my_turn = empty + S::kStages, *const of_half = my_turn + H;
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(of_half + H * S::kHalfBarriers);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             ofd::mbar_init(&full[i], 1);
             ofd::mbar_init(&empty[i], H);
         }
+        for (int i = 0; i < H; ++i) ofd::mbar_init(&my_turn[i], 1);
         for (int i = 0; i < H * S::kHalfBarriers; ++i) {
             // s_full and o_done are a commit's, p_ready and q_ready take an arrival of each warp
             const int of = i % S::kHalfBarriers;
@@ -291,6 +292,9 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                 }
                 fine = fine && tc5::wait_warp(&p_ready[buffer], (i - S::kBuffers) / S::kBuffers & 1, given_up, &g_status);
             }
+            // The halves take turns, so that one's weights are worked out beside the other's products: both at once end
+            // together, and then the matrix unit has nothing to do.
+            if (H == 2) fine = fine && tc5::wait_warp(&my_turn[x], (step + x + 1) & 1, given_up, &g_status);
             tc5::after_sync();
             if (fine && tc5::elect()) {
                 if (sums) {
@@ -310,6 +314,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                 } else if (sums) {
                     tc5::commit(&o_done[step - end]);  // the last ones, which no S follows
                 }
+                if (H == 2) tc5::arrive(&my_turn[x ^ 1]);
                 if (S::kCopyWarp) tc5::commit(&empty[stage]);
                 // The weights were there, so S before them was: the products of the last step are done.
                 else if (step > 0 && step + S::kStages - 1 < steps) load(step + S::kStages - 1, stage == 0 ? S::kStages - 1 : stage - 1);
