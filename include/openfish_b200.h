@@ -254,10 +254,7 @@ typedef struct openfish_b200_matmul_i8 {
     const void *bias; /* or NULL */
     void *out;
     long long x_stride, w_stride, out_stride;
-    void *workspace; /* 16-byte aligned; NULL where openfish_b200_matmul_i8_workspace says 0 */
-    size_t workspace_bytes;
 } openfish_b200_matmul_i8_t;
-size_t openfish_b200_matmul_i8_workspace(const openfish_b200_matmul_i8_t *args);
 void openfish_b200_matmul_i8(void *cuda_stream, const openfish_b200_matmul_i8_t *args);
 
 /* Residual, norm and 8-bit tokens, row by row:

@@ -308,5 +308,5 @@ def last_rotary_ms():
     return float(lib().openfish_b200_last_rotary_ms())
 
 
-from .encoder import attention, encoder_wait, matmul_i8, norm, quantize_i8  # noqa: E402,F401
+from .encoder import attention, attention_workspace_bytes, encoder_wait, matmul_i8, norm, quantize_i8  # noqa: E402,F401
 from .sharding import shard_range  # noqa: E402,F401

@@ -13,7 +13,6 @@ extern "C" {
 int ofb_attention(void *stream, const openfish_b200_attention_t *a);
 size_t ofb_attention_workspace(const openfish_b200_attention_t *a);
 int ofb_matmul_i8(void *stream, const openfish_b200_matmul_i8_t *a);
-size_t ofb_matmul_i8_workspace(const openfish_b200_matmul_i8_t *a);
 int ofb_norm(void *stream, const openfish_b200_norm_t *a);
 /* Waits for the stream; then *gave_up: whether a kernel of the file has given up a wait on this device since the last call. */
 int ofb_attention_settle(void *stream, int *gave_up);

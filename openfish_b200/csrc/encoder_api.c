@@ -102,12 +102,6 @@ static int bad_matmul_sizes(const char *func, const openfish_b200_matmul_i8_t *a
     return 0;
 }
 
-size_t openfish_b200_matmul_i8_workspace(const openfish_b200_matmul_i8_t *args) {
-    ofb_api_clear();
-    if (bad_matmul_sizes(__func__, args) || args->rows == 0) return 0;
-    return ofb_matmul_i8_workspace(args);
-}
-
 void openfish_b200_matmul_i8(void *cuda_stream, const openfish_b200_matmul_i8_t *a) {
     ofb_api_clear();
     if (bad_matmul_sizes(__func__, a) || a->rows == 0) return;
@@ -123,13 +117,6 @@ void openfish_b200_matmul_i8(void *cuda_stream, const openfish_b200_matmul_i8_t 
     if (!aligned(a->x_scale, 4) || !aligned(a->w_scale, 4) || !aligned(a->out, 2) || !aligned(a->bias, 2) ||
         (a->rows > 1 && a->out_stride < a->cols) || a->x_stride > (1LL << 38) || a->w_stride > (1LL << 38) || a->out_stride > (1LL << 37)) {
         refuse(__func__, OPENFISH_B200_ERR_LAYOUT, "scales, bias and out must be aligned to their types, rows of out cols or more apart");
-        return;
-    }
-    const size_t need = ofb_matmul_i8_workspace(a);
-    if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16))) {
-        char msg[160];
-        snprintf(msg, sizeof(msg), "needs a 16-byte aligned workspace of %zu bytes (openfish_b200_matmul_i8_workspace)", need);
-        refuse(__func__, OPENFISH_B200_ERR_ARGUMENT, msg);
         return;
     }
     ofb_api_backend_failed(__func__, ofb_matmul_i8(cuda_stream, a));

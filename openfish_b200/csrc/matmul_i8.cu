@@ -329,8 +329,6 @@ int run(const Args &a, int sms, cudaStream_t stream) {
 
 }  // namespace
 
-extern "C" size_t ofb_matmul_i8_workspace(const openfish_b200_matmul_i8_t *) { return 0; }
-
 extern "C" int ofb_matmul_i8(void *stream, const openfish_b200_matmul_i8_t *p) {
     int sms = 0;
     if (const int rc = ofe::sm_count(&sms)) return rc;

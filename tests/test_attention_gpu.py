@@ -283,8 +283,7 @@ def test_captured_and_on_two_streams_at_once(native_lib, q_len, k_len):
 def test_the_workspace_is_asked_for_and_checked(native_lib):
     q, k, v = make(1, 8, 64, torch.float16, 1), make(30000, 2, 64, torch.float16, 2), make(30000, 2, 64, torch.float16, 3)
     a, b = starts([1])[1], starts([30000])[1]
-    out = torch.empty_like(q)
-    need = native_lib.encoder.attention_workspace_bytes(native_lib.encoder.attention_args(q, k, v, a, b, 1, 30000, out))
+    need = native_lib.attention_workspace_bytes(q, k, v, a, b, 1, 30000)
     want = native_lib.attention(q, k, v, a, b, 1, 30000)
     if need:
         with pytest.raises(native_lib.OpenfishError):
