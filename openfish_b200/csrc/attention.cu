@@ -26,6 +26,10 @@
 
 namespace {
 
+using ofe::add2;
+using ofe::fma2;
+using ofe::pack;
+
 __device__ int g_status;  // of the kernels on this device: a wait that ran out
 
 constexpr int kRows = 128;  // of a half
@@ -72,33 +76,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// Two fp32 operations in an instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 y;
-    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%6, %7};\n\t"
-        "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
-        : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return y;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 y;
-    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
-        : "=f"(y.x), "=f"(y.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return y;
-}
-template <class T>
-__device__ __forceinline__ uint32_t pack(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // Two weights 2^(c s - c m) as the matrix unit takes them, added to their row's sum (before they are rounded).
 template <class T>
 __device__ __forceinline__ uint32_t weights(float u, float w, float c, float shift, float2 &sum) {

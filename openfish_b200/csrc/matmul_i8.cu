@@ -27,15 +27,18 @@ struct Args {
 // Tiles of 128 * CG tokens by BN channels.  CG = 2: a pair of blocks on two neighbouring SMs shares one tile, each holding half of
 // the tokens and half of the channels' weights, so that a byte of shared memory is filled once and read by both.
 //
-// Warps: 0 issues the copies, 1 the matrix instructions, 4 to 7 (a quarter of the accumulator's 128 lanes each) scale and
-// store.  The accumulator is there twice, so that one tile's sums are stored while the next one's are formed.
+// Warps: 0 issues the copies, 1 the matrix instructions, the ones from 4 on (a quarter of the accumulator's 128 lanes and half
+// of its columns each) scale and store.  The accumulator is there twice, so that one tile's sums are stored while the next one's are
+// formed; the scales of a tile are fetched while the last one is stored.
 template <int CG, int BN>
 struct Shape {
     static constexpr int kRowsB = BN / CG;                     // weights' rows in one block
     static constexpr int kStageBytes = (128 + kRowsB) * 128;   // 128 deep
-    static constexpr int kStages = BN == 64 ? 7 : 5;
-    static constexpr int kOutBytes = 4 * 2 * 4096;             // a warp's 32 rows of 64 results, twice
-    static constexpr int kScaleBytes = 4 * 64 * 8;             // a warp's 64 channel scales and biases
+    static constexpr int kParts = BN >= 128 ? 2 : 1, kPart = BN / kParts;  // of a tile's columns, each with its four warps
+    static constexpr int kThreads = 128 + 128 * kParts;
+    static constexpr int kStages = BN == 64 ? 7 : 4;
+    static constexpr int kOutBytes = kParts * 4 * 2 * 4096;    // a warp's 32 rows of 64 results, twice
+    static constexpr int kScaleBytes = kParts * 4 * kPart * 8; // a warp's channel scales and biases
     static constexpr int kBytes = 1024 + kStages * kStageBytes + kOutBytes + kScaleBytes + (2 * kStages + 5) * 8 + 8;
     static constexpr int kColumns = 2 * BN;                    // of tensor memory, a power of two
 };
@@ -51,8 +54,8 @@ struct Walk {  // the tiles in the order in which they are taken: stripes of 8 t
 };
 
 template <class T, int CG, int BN>
-__global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
-                                                           const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
+__global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
+                                                                                 const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<CG, BN>;
     extern __shared__ uint8_t raw[];
     uint8_t *const base = raw + ((1024 - (tc5::smem_u32(raw) & 1023)) & 1023);
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const
         }
         for (int i = 0; i < 2; ++i) {
             ofd::mbar_init(&sum_full[i], 1);
-            ofd::mbar_init(&sum_empty[i], 4 * CG);
+            ofd::mbar_init(&sum_empty[i], 4 * S::kParts * CG);
         }
         ofd::mbar_init(done, 1);
         ofd::mbar_fence_init();
@@ -150,50 +153,61 @@ __global__ void __launch_bounds__(256, 1) matmul_tile_kernel(const Args a, const
             ofd::mbar_land(done, 0, 0, ofd::kDefaultWaitLimitNs);
         }
     } else if (warp >= 4) {
-        const int quarter = warp & 3;
-        uint8_t *const mine = out_stage + quarter * 8192;
-        float2 *const scales = scale_stage + quarter * 64;
+        const int quarter = warp & 3, part = (warp - 4) >> 2;
+        uint8_t *const mine = out_stage + (warp - 4) * 8192;
+        float2 *const scales = scale_stage + (warp - 4) * S::kPart;
         const T *const bias = static_cast<const T *>(a.bias);
+        float2 next[S::kPart / 32];  // the next tile's scales and biases, a lane to a column
+        float next_xs = 0.f;
+        const auto fetch = [&](int t) {
+            int tm, tn;
+            walk.at(t, &tm, &tn);
+            const int m = tm * 128 * CG + rank * 128 + quarter * 32 + lane, n0 = tn * BN + part * S::kPart;
+            next_xs = t < tiles && m < a.rows ? a.x_scale[m] : 0.f;
+#pragma unroll
+            for (int i = 0; i < S::kPart / 32; ++i) {
+                const int n = n0 + i * 32 + lane;
+                const bool in = t < tiles && n < a.cols;
+                next[i].x = in ? a.w_scale[n] : 0.f;
+                next[i].y = in && bias ? ofe::to_float(bias[n]) : 0.f;
+            }
+        };
+        fetch(group);
         int j = 0, turn = 0;
         for (int t = group; t < tiles; t += groups, ++j) {
             int tm, tn;
             walk.at(t, &tm, &tn);
-            const int m0 = tm * 128 * CG + rank * 128 + quarter * 32, n0 = tn * BN;
-            const float xs = m0 + lane < a.rows ? a.x_scale[m0 + lane] : 0.f;
+            const int m0 = tm * 128 * CG + rank * 128 + quarter * 32, n0 = tn * BN + part * S::kPart;
+            const float xs = next_xs;
+            __syncwarp();  // the last tile's scales have been read
+#pragma unroll
+            for (int i = 0; i < S::kPart / 32; ++i) scales[i * 32 + lane] = next[i];
+            __syncwarp();
+            fetch(t + groups);
             if (!tc5::wait_warp(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status)) break;
             tc5::after_sync();
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 64, ++turn) {
-                const uint32_t sum = tmem + ((uint32_t)(quarter * 32) << 16) + (j & 1) * BN + c;
+            for (int c = 0; c < S::kPart; c += 64, ++turn) {
+                const uint32_t sum = tmem + ((uint32_t)(quarter * 32) << 16) + (j & 1) * BN + part * S::kPart + c;
                 uint32_t v[2][32];
-                __syncwarp();
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int n = n0 + c + h * 32 + lane;
-                    float2 sb = {0.f, 0.f};
-                    if (n < a.cols) {
-                        sb.x = a.w_scale[n];
-                        if (bias) sb.y = ofe::to_float(bias[n]);
-                    }
-                    scales[h * 32 + lane] = sb;
-                }
-                if (lane == 0) tc5::store_wait_read<1>();  // the copy out of this half of the staging memory is done with it
-                __syncwarp();
                 tc5::ld64(v[0], v[1], sum);
-                if (c + 64 >= BN) {  // the accumulator has been read: the next tile's sums may go there
+                if (c + 64 >= S::kPart) {  // the accumulator has been read: the next tile's sums may go there
                     tc5::before_sync();
+                    __syncwarp();
                     if (lane == 0) {
                         if (CG == 1) tc5::arrive(&sum_empty[j & 1]);
                         else tc5::arrive_cluster(tc5::of_first_block(tc5::smem_u32(&sum_empty[j & 1])));
                     }
                 }
+                if (lane == 0) tc5::store_wait_read<1>();  // the copy out of this half of the staging memory is done with it
+                __syncwarp();
                 uint8_t *const to = mine + (turn & 1) * 4096;
 #pragma unroll
                 for (int p = 0; p < 8; ++p) {
                     alignas(16) T o[8];
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        const float4 sb = reinterpret_cast<const float4 *>(scales)[p * 4 + e / 2];
+                        const float4 sb = reinterpret_cast<const float4 *>(scales + c)[p * 4 + e / 2];
                         const int at = (p & 3) * 8 + e;
                         o[e] = ofe::from_float<T>(fmaf((float)(int)v[p >> 2][at], xs * sb.x, sb.y));
                         o[e + 1] = ofe::from_float<T>(fmaf((float)(int)v[p >> 2][at + 1], xs * sb.z, sb.w));
@@ -256,7 +270,7 @@ int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
     const int most = sms / CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

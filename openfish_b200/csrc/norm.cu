@@ -17,7 +17,10 @@
 
 namespace {
 
+using ofe::add2;
+using ofe::fma2;
 using ofe::from_float;
+using ofe::mul2;
 using ofe::to_float;
 
 template <class T>
@@ -31,15 +34,28 @@ struct NormArgs {
     float eps, alpha;
 };
 
-// V elements that lie together: 16 bytes where everything is aligned to that, else one at a time.
+// V elements that lie together, two at a time: 16 bytes where everything is aligned to that, else one element (and a
+// zero beside it).
 template <class T, int V>
-struct alignas(V == 8 ? 16 : sizeof(T)) Pack {
-    T v[V];
-};
-template <int V>
-struct alignas(V) Pack8 {
-    int8_t v[V];
-};
+__device__ __forceinline__ void read(const T *p, float2 (&f)[(V + 1) / 2]) {
+    if (V == 8) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        f[0] = ofe::unpack<T>(w.x);
+        f[V / 8] = ofe::unpack<T>(w.y);
+        f[V / 4] = ofe::unpack<T>(w.z);
+        f[V / 8 * 3] = ofe::unpack<T>(w.w);
+    } else {
+        f[0] = make_float2(to_float(*p), 0.f);
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void write(T *p, const float2 (&f)[(V + 1) / 2]) {
+    if (V == 8)
+        *reinterpret_cast<uint4 *>(p) = make_uint4(ofe::pack<T>(f[0].x, f[0].y), ofe::pack<T>(f[V / 8].x, f[V / 8].y),
+                                                   ofe::pack<T>(f[V / 4].x, f[V / 4].y), ofe::pack<T>(f[V / 8 * 3].x, f[V / 8 * 3].y));
+    else
+        *p = from_float<T>(f[0].x);
+}
 
 // A sum (or maximum) over the threads of a row: its warp, or all warps of the block through shared memory.
 template <bool BLOCK, class Op>
@@ -72,100 +88,109 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
     const auto most = [](float p, float q) { return fmaxf(p, q); };
     const float inv = 1.f / (float)a.width;
 
+    constexpr int P = (V + 1) / 2;
     for (long long row = first; row < a.rows; row += step) {
-        const T *x = a.x + row * a.x_stride;
-        const T *r = a.r ? a.r + row * a.r_stride : nullptr;
-        float s[CH][V];
-        Pack<T, V> px[CH], pr[CH];
+        const T *const x = a.x + row * a.x_stride, *const r = a.r + row * a.r_stride;
+        float2 s[CH][P];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int at = (c * lanes + lane) * V;
-            if (at < a.width) {
-                px[c] = *reinterpret_cast<const Pack<T, V> *>(x + at);
-                if (r) pr[c] = *reinterpret_cast<const Pack<T, V> *>(r + at);
-            }
-        }
-        float sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const bool in = (c * lanes + lane) * V < a.width;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float f = in ? to_float(px[c].v[i]) : 0.f;
-                if (r && in) f = fmaf(a.alpha, to_float(pr[c].v[i]), f);
-                s[c][i] = f;
-                sum += f;
-            }
+            for (int i = 0; i < P; ++i) s[c][i] = {0.f, 0.f};
+            if (at < a.width) read<T, V>(x + at, s[c]);
         }
-        float mean = 0.f, factor = 1.f;
-        if (a.kind != OPENFISH_B200_NORM_NONE) {
-            if (a.kind == OPENFISH_B200_NORM_LAYER) mean = reduce<BLOCK>(sum, scratch, add) * inv;
-            float sq = 0.f;
+        if (a.r) {
+            float2 f[CH][P];
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const bool in = (c * lanes + lane) * V < a.width;
+                const int at = (c * lanes + lane) * V;
+                if (at < a.width) {
+                    read<T, V>(r + at, f[c]);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = s[c][i] - mean;
-                    if (in) sq = fmaf(d, d, sq);
+                    for (int i = 0; i < P; ++i) s[c][i] = fma2(f[c][i], {a.alpha, a.alpha}, s[c][i]);
                 }
             }
-            factor = 1.f / sqrtf(reduce<BLOCK>(sq, scratch, add) * inv + a.eps);
         }
-        float top = 0.f;
-        bool odd = false;  // an infinity or NaN in the row
+        if (a.kind != OPENFISH_B200_NORM_NONE) {
+            float2 sum = {0.f, 0.f};
+            if (a.kind == OPENFISH_B200_NORM_LAYER) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int at = (c * lanes + lane) * V;
-            if (at < a.width) {
-                if (a.kind != OPENFISH_B200_NORM_NONE) {
-                    Pack<T, V> w, b;
-                    if (a.w) w = *reinterpret_cast<const Pack<T, V> *>(a.w + at);
-                    if (a.b) b = *reinterpret_cast<const Pack<T, V> *>(a.b + at);
+                for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        float y = (s[c][i] - mean) * factor;
-                        if (a.w) y *= to_float(w.v[i]);
-                        if (a.b) y += to_float(b.v[i]);
-                        s[c][i] = y;
+                    for (int i = 0; i < P; ++i) sum = add2(sum, s[c][i]);
+                const float mean = reduce<BLOCK>(sum.x + sum.y, scratch, add) * inv;
+                sum = {0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    if ((c * lanes + lane) * V < a.width) {
+#pragma unroll
+                        for (int i = 0; i < P; ++i) s[c][i] = add2(s[c][i], {-mean, V == 1 ? 0.f : -mean});
                     }
                 }
-                if (a.out) {
-                    Pack<T, V> o;
+            }
 #pragma unroll
-                    for (int i = 0; i < V; ++i) o.v[i] = from_float<T>(s[c][i]);
-                    *reinterpret_cast<Pack<T, V> *>(a.out + row * a.out_stride + at) = o;
-                }
+            for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    top = fmaxf(top, fabsf(s[c][i]));
-                    odd |= !(fabsf(s[c][i]) < INFINITY);
+                for (int i = 0; i < P; ++i) sum = fma2(s[c][i], s[c][i], sum);
+            const float factor = 1.f / sqrtf(reduce<BLOCK>(sum.x + sum.y, scratch, add) * inv + a.eps);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int at = (c * lanes + lane) * V;
+                if (at < a.width) {
+                    float2 f[P];
+#pragma unroll
+                    for (int i = 0; i < P; ++i) s[c][i] = mul2(s[c][i], {factor, factor});
+                    if (a.w) {
+                        read<T, V>(a.w + at, f);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) s[c][i] = mul2(s[c][i], f[i]);
+                    }
+                    if (a.b) {
+                        read<T, V>(a.b + at, f);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) s[c][i] = add2(s[c][i], f[i]);
+                    }
                 }
+            }
+        }
+        if (a.out) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int at = (c * lanes + lane) * V;
+                if (at < a.width) write<T, V>(a.out + row * a.out_stride + at, s[c]);
             }
         }
         if (!a.q) continue;
-        // (fmaxf drops a NaN; such a row counts as one with an infinity)
+        float top = 0.f;
+        bool odd = false;  // an infinity or NaN in the row (a NaN is lost on a maximum; such a row counts as one with an infinity)
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                top = fmaxf(top, fmaxf(fabsf(s[c][i].x), fabsf(s[c][i].y)));
+                odd |= !(fabsf(s[c][i].x) < INFINITY) | !(fabsf(s[c][i].y) < INFINITY);
+            }
         top = reduce<BLOCK>(odd ? INFINITY : top, scratch, most);
         const bool fine = top < INFINITY;
-        const float scale = top / 127.f;
-        // y * (127 / top) may miss y / scale by an ulp, which moves a value that lies on the border of two steps.  A
-        // top so small that 127 / top overflows is divided by.
-        const float back = 127.f / top;
+        const float back = 127.f / top;  // no number for a row of zeros, and beyond fp32 for one whose top is below 2^-121
         const bool direct = back < INFINITY;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int at = (c * lanes + lane) * V;
             if (at < a.width) {
-                Pack8<V> o;
+                alignas(8) int8_t o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float f = !fine || top == 0.f ? 0.f : direct ? s[c][i] * back : s[c][i] / top * 127.f;
-                    o.v[i] = (int8_t)max(-127, min(127, __float2int_rn(f)));
+                    const float y = i & 1 ? s[c][i / 2].y : s[c][i / 2].x;
+                    const float f = direct ? y * back : top > 0.f ? y / top * 127.f : 0.f;
+                    // (|f| is at most 127 and a rounding: no clamp can be reached)
+                    o[i] = fine ? (int8_t)__float2int_rn(f) : (int8_t)0;
                 }
-                *reinterpret_cast<Pack8<V> *>(a.q + row * a.q_stride + at) = o;
+                if (V == 8) *reinterpret_cast<uint2 *>(a.q + row * a.q_stride + at) = *reinterpret_cast<const uint2 *>(o);
+                else a.q[row * a.q_stride + at] = o[0];
             }
         }
-        if (lane == 0) a.q_scale[row] = fine ? scale : NAN;
+        if (lane == 0) a.q_scale[row] = fine ? top / 127.f : NAN;
     }
 }
 
@@ -173,7 +198,9 @@ template <class T, int V, int CH, bool BLOCK>
 void launch(const NormArgs<T> &a, int threads, int sms, cudaStream_t stream) {
     const long long per_block = BLOCK ? 1 : threads / 32;
     long long blocks = (a.rows + per_block - 1) / per_block;
-    const long long cap = (long long)sms * (2048 / threads) * 4;
+    // Up to 32 warps to a scheduler's worth of rows in turn (53312 rows of 512 with a residual, us by blocks of full occupancy: one 32.2, two 31.1,
+    // four 32.0, a block to four rows 32.8).
+    const long long cap = (long long)sms * (2048 / threads) * 2;
     if (blocks > cap) blocks = cap;
     norm_kernel<T, V, CH, BLOCK><<<(unsigned)blocks, threads, 0, stream>>>(a);
 }
