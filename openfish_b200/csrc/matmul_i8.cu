@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
     extern __shared__ uint8_t raw[];
     uint8_t *const base = raw + ((1024 - (tc5::smem_u32(raw) & 1023)) & 1023);
     uint8_t *const out_stage = base + S::kStages * S::kStageBytes;
-    float2 *const scale_stage = reinterpret_cast<float2 *>(out_stage + S::kOutBytes);
+    float *const scale_stage = reinterpret_cast<float *>(out_stage + S::kOutBytes);
     uint64_t *const full = reinterpret_cast<uint64_t *>(out_stage + S::kOutBytes + S::kScaleBytes);
     uint64_t *const empty = full + S::kStages, *const sum_full = empty + S::kStages, *const sum_empty = sum_full + 2, *const done = sum_empty + 2;
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
     } else if (warp >= 4) {
         const int quarter = warp & 3, part = (warp - 4) >> 2;
         uint8_t *const mine = out_stage + (warp - 4) * 8192;
-        float2 *const scales = scale_stage + (warp - 4) * S::kPart;
+        float *const scales = scale_stage + (warp - 4) * 2 * S::kPart, *const biases = scales + S::kPart;
         const T *const bias = static_cast<const T *>(a.bias);
         float2 next[S::kPart / 32];  // the next tile's scales and biases, a lane to a column
         float next_xs = 0.f;
@@ -181,7 +181,10 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
             const float xs = next_xs;
             __syncwarp();  // the last tile's scales have been read
 #pragma unroll
-            for (int i = 0; i < S::kPart / 32; ++i) scales[i * 32 + lane] = next[i];
+            for (int i = 0; i < S::kPart / 32; ++i) {
+                scales[i * 32 + lane] = next[i].x;
+                biases[i * 32 + lane] = next[i].y;
+            }
             __syncwarp();
             fetch(t + groups);
             if (!tc5::wait_warp(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status)) break;
@@ -203,16 +206,20 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                 __syncwarp();
                 uint8_t *const to = mine + (turn & 1) * 4096;
 #pragma unroll
-                for (int p = 0; p < 8; ++p) {
-                    alignas(16) T o[8];
+                for (int p = 0; p < 8; ++p) {  // eight results, two to an instruction
+                    uint32_t o[4];
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const float4 sb = reinterpret_cast<const float4 *>(scales + c)[p * 4 + e / 2];
-                        const int at = (p & 3) * 8 + e;
-                        o[e] = ofe::from_float<T>(fmaf((float)(int)v[p >> 2][at], xs * sb.x, sb.y));
-                        o[e + 1] = ofe::from_float<T>(fmaf((float)(int)v[p >> 2][at + 1], xs * sb.z, sb.w));
+                    for (int e = 0; e < 4; e += 2) {
+                        const float4 sw = *reinterpret_cast<const float4 *>(scales + c + p * 8 + e * 2);
+                        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (bias) b = *reinterpret_cast<const float4 *>(biases + c + p * 8 + e * 2);
+                        const uint32_t *const sum4 = &v[p >> 2][(p & 3) * 8 + e * 2];
+                        const float2 lo = ofe::fma2(ofe::mul2(make_float2((float)(int)sum4[0], (float)(int)sum4[1]), {xs, xs}), {sw.x, sw.y}, {b.x, b.y});
+                        const float2 hi = ofe::fma2(ofe::mul2(make_float2((float)(int)sum4[2], (float)(int)sum4[3]), {xs, xs}), {sw.z, sw.w}, {b.z, b.w});
+                        o[e] = ofe::pack<T>(lo.x, lo.y);
+                        o[e + 1] = ofe::pack<T>(hi.x, hi.y);
                     }
-                    *reinterpret_cast<uint4 *>(to + lane * 128 + ((p ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(o);
+                    *reinterpret_cast<uint4 *>(to + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
                 if (a.by_copy) {
                     tc5::fence_async();

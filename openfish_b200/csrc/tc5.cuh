@@ -49,8 +49,9 @@ __device__ __forceinline__ uint32_t of_first_block(uint32_t addr) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(addr));
     return at;
 }
+// (no memory is handed over with it, only tensor memory, which has fences of its own: nothing to release)
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
