@@ -95,59 +95,65 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
     tc5::after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         // copies: each block its own rows; the bytes of both are counted at the first block's barrier
-        int i = 0;
+        int stage = 0, issued = 0;
+        uint32_t turn = 0;
         bool fine = true;
         for (int t = group; t < tiles && fine; t += groups) {
             int tm, tn;
             walk.at(t, &tm, &tn);
             const int m = tm * 128 * CG + rank * 128, n = tn * BN + rank * S::kRowsB;
-            for (int k = 0; k < steps; ++k, ++i) {
-                const int s = i % S::kStages;
-                fine = tc5::wait(&empty[s], ((i / S::kStages) & 1) ^ 1, given_up, &g_status);
+            for (int k = 0; k < steps; ++k, ++issued) {
+                fine = tc5::wait_warp(&empty[stage], turn ^ 1, given_up, &g_status);
                 if (!fine) break;
-                uint8_t *const to = base + s * S::kStageBytes;
-                if (CG == 1) {
-                    ofd::mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-                    tc5::load_2d(to, &map_x, k * 128, m, &full[s]);
-                    tc5::load_2d(to + 128 * 128, &map_w, k * 128, n, &full[s]);
-                } else {
-                    if (rank == 0) ofd::mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);
-                    const uint32_t bar = tc5::of_first_block(tc5::smem_u32(&full[s]));
-                    tc5::load_2d_pair(to, &map_x, k * 128, m, bar);
-                    tc5::load_2d_pair(to + 128 * 128, &map_w, k * 128, n, bar);
+                uint8_t *const to = base + stage * S::kStageBytes;
+                if (tc5::elect()) {
+                    if (CG == 1) {
+                        ofd::mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
+                        tc5::load_2d(to, &map_x, k * 128, m, &full[stage]);
+                        tc5::load_2d(to + 128 * 128, &map_w, k * 128, n, &full[stage]);
+                    } else {
+                        if (rank == 0) ofd::mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
+                        const uint32_t bar = tc5::of_first_block(tc5::smem_u32(&full[stage]));
+                        tc5::load_2d_pair(to, &map_x, k * 128, m, bar);
+                        tc5::load_2d_pair(to + 128 * 128, &map_w, k * 128, n, bar);
+                    }
                 }
+                __syncwarp();
+                if (++stage == S::kStages) stage = 0, turn ^= 1;
             }
         }
         // after a wait that ran out: the copies under way land before the block ends
-        if (!fine && rank == 0) ofd::mbar_drain_bounded(full, S::kStages, i, ofd::kDefaultWaitLimitNs);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+        if (!fine && rank == 0 && lane == 0) ofd::mbar_drain_bounded(full, S::kStages, issued, ofd::kDefaultWaitLimitNs);
+    } else if (warp == 1 && rank == 0) {
         constexpr uint32_t idesc = tc5::idesc_i8(128 * CG, BN);
-        int i = 0, j = 0;
+        const uint64_t base_a = tc5::desc_k_major(tc5::smem_u32(base)), base_b = tc5::desc_k_major(tc5::smem_u32(base) + 128 * 128);
+        int stage = 0, j = 0;
+        uint32_t turn = 0;
         bool fine = true;
         for (int t = group; t < tiles && fine; t += groups, ++j) {
             const uint32_t sum = tmem + (j & 1) * BN;
-            fine = tc5::wait(&sum_empty[j & 1], ((j >> 1) & 1) ^ 1, given_up, &g_status);
-            if (!fine) break;
-            tc5::after_sync();
-            for (int k = 0; k < steps; ++k, ++i) {
-                const int s = i % S::kStages;
-                fine = tc5::wait(&full[s], (i / S::kStages) & 1, given_up, &g_status);
-                if (!fine) break;
+            fine = tc5::wait_warp(&sum_empty[j & 1], ((j >> 1) & 1) ^ 1, given_up, &g_status);
+            for (int k = 0; k < steps && fine; ++k) {
+                fine = tc5::wait_warp(&full[stage], turn, given_up, &g_status);
                 tc5::after_sync();
-                const uint32_t at = tc5::smem_u32(base + s * S::kStageBytes);
-                const uint64_t da = tc5::desc_k_major(at), db = tc5::desc_k_major(at + 128 * 128);
+                const uint64_t da = base_a + (uint32_t)(stage * (S::kStageBytes >> 4)), db = base_b + (uint32_t)(stage * (S::kStageBytes >> 4));
+                if (fine && tc5::elect()) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) tc5::mma_i8<CG>(sum, da + 2 * q, db + 2 * q, idesc, (k | q) != 0);
-                if (CG == 1) tc5::commit(&empty[s]);
-                else tc5::commit_pair(&empty[s]);
+                    for (int q = 0; q < 4; ++q) tc5::mma_i8<CG>(sum, da + 2 * q, db + 2 * q, idesc, k > 0 || q > 0);
+                    if (CG == 1) tc5::commit(&empty[stage]);
+                    else tc5::commit_pair(&empty[stage]);
+                    if (k + 1 == steps) {
+                        if (CG == 1) tc5::commit(&sum_full[j & 1]);
+                        else tc5::commit_pair(&sum_full[j & 1]);
+                    }
+                }
+                __syncwarp();
+                if (++stage == S::kStages) stage = 0, turn ^= 1;
             }
-            if (!fine) break;
-            if (CG == 1) tc5::commit(&sum_full[j & 1]);
-            else tc5::commit_pair(&sum_full[j & 1]);
         }
-        if (!fine) {  // after a wait that ran out: the instructions under way end before the block does
+        if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
             if (CG == 1) tc5::commit(done);
             else tc5::commit_pair(done);
             ofd::mbar_land(done, 0, 0, ofd::kDefaultWaitLimitNs);
