@@ -36,8 +36,8 @@ struct Shape {
     static constexpr int kStageBytes = (128 + kRowsB) * 128;   // 128 deep
     static constexpr int kParts = BN >= 128 ? 2 : 1, kPart = BN / kParts;  // of a tile's columns, each with its four warps
     static constexpr int kThreads = 128 + 128 * kParts;
-    static constexpr int kStages = BN == 64 ? 7 : 4;
-    static constexpr int kOutBytes = kParts * 4 * 2 * 4096;    // a warp's 32 rows of 64 results, twice
+    static constexpr int kStages = BN == 64 ? 7 : 5;
+    static constexpr int kOutBytes = kParts * 4 * 4096;    // a warp's 32 rows of 64 results, twice
     static constexpr int kScaleBytes = kParts * 4 * kPart * 8; // a warp's channel scales and biases
     static constexpr int kBytes = 1024 + kStages * kStageBytes + kOutBytes + kScaleBytes + (2 * kStages + 5) * 8 + 8;
     static constexpr int kColumns = 2 * BN;                    // of tensor memory, a power of two
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, part = (warp - 4) >> 2;
-        uint8_t *const mine = out_stage + (warp - 4) * 8192;
+        uint8_t *const mine = out_stage + (warp - 4) * 4096;
         float *const scales = scale_stage + (warp - 4) * 2 * S::kPart, *const biases = scales + S::kPart;
         const T *const bias = static_cast<const T *>(a.bias);
         float2 next[S::kPart / 32];  // the next tile's scales and biases, a lane to a column
@@ -208,9 +208,9 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                         else tc5::arrive_cluster(tc5::of_first_block(tc5::smem_u32(&sum_empty[j & 1])));
                     }
                 }
-                if (lane == 0) tc5::store_wait_read<1>();  // the copy out of this half of the staging memory is done with it
+                if (lane == 0) tc5::store_wait_read<0>();  // the copy out of this half of the staging memory is done with it
                 __syncwarp();
-                uint8_t *const to = mine + (turn & 1) * 4096;
+                uint8_t *const to = mine;
 #pragma unroll
                 for (int p = 0; p < 8; ++p) {  // eight results, two to an instruction
                     uint32_t o[4];
