@@ -43,7 +43,7 @@ struct Args {
     float *part, *part_lse;  // of a split: [split][q_rows][q_heads][head_dim] and [split][q_rows][q_heads]
     long long q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head, out_stride_row, out_stride_head;
     int q_rows, k_rows, q_heads, kv_heads, group, head_dim, sequences, max_q, max_k, left, right;
-    uint32_t group_mul, group_shift;  // r / group = (mulhi(r, group_mul) + r) >> group_shift for r < 2^30
+    ofe::Divider by_group;
     int tiles, splits;  // blocks of rows to the longest sequence; pieces of a block's keys
     float c;
 };
@@ -62,8 +62,6 @@ __device__ __forceinline__ void window(const Args &a, int i, int nq, int nk, int
     *lo = a.left < 0 ? 0 : max(place - a.left, 0);
     *hi = a.right < 0 ? nk : min(place + a.right + 1, nk);
 }
-
-__device__ __forceinline__ int by_group(const Args &a, int r) { return (int)((__umulhi((uint32_t)r, a.group_mul) + (uint32_t)r) >> a.group_shift); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -165,8 +163,8 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
         int unused;
         lo[x] = hi[x] = 0;
         if (r0 + x * kRows >= rows) continue;
-        window(a, by_group(a, r0 + x * kRows), nq, nk, &lo[x], &unused);
-        window(a, by_group(a, min(r0 + (x + 1) * kRows, rows) - 1), nq, nk, &unused, &hi[x]);
+        window(a, a.by_group.quotient(r0 + x * kRows), nq, nk, &lo[x], &unused);
+        window(a, a.by_group.quotient(min(r0 + (x + 1) * kRows, rows) - 1), nq, nk, &unused, &hi[x]);
         if (hi[x] <= lo[x]) continue;
         all_lo = all_hi == 0 ? lo[x] : min(all_lo, lo[x]);
         all_hi = max(all_hi, hi[x]);
@@ -306,14 +304,14 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     } else {
         const int begin = H == 1 ? 0 : from[x], end = H == 1 ? count : to[x];
         const int row = (warp & 3) * 32 + lane, half0 = r0 + x * kRows;  // of the half, and lane of tensor memory; the half's first
-        const int r = half0 + row, i = by_group(a, r), head = kh * a.group + r - i * a.group;
+        const int r = half0 + row, i = a.by_group.quotient(r), head = kh * a.group + r - i * a.group;
         const bool there = r < rows, warp_there = half0 + (warp & 3) * 32 < rows;
         // ---- the queries into shared memory, pieces of 16 bytes; zeros where there are none
         if (end > begin) {
             constexpr int kPieces = DP / 8;
 #pragma unroll 4
             for (int n = threadIdx.x & 127; n < kRows * kPieces; n += 128) {
-                const int qr = n / kPieces, p = n % kPieces, rr = half0 + qr, ri = by_group(a, rr);
+                const int qr = n / kPieces, p = n % kPieces, rr = half0 + qr, ri = a.by_group.quotient(rr);
                 uint4 val = make_uint4(0, 0, 0, 0);
                 if (rr < rows && p * 8 < a.head_dim)
                     val = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(q0 + ri) * a.q_stride_row +
@@ -327,7 +325,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
         // ---- the keys this row sees, and between them the first and the last row of the warp (rows that are not there
         // are given the last row's)
         int my_lo, my_hi;
-        window(a, by_group(a, min(r, rows - 1)), nq, nk, &my_lo, &my_hi);
+        window(a, a.by_group.quotient(min(r, rows - 1)), nq, nk, &my_lo, &my_hi);
         const int first_lo = __shfl_sync(0xffffffffu, my_lo, 0), first_hi = __shfl_sync(0xffffffffu, my_hi, 0);
         const int last_lo = __shfl_sync(0xffffffffu, my_lo, 31), last_hi = __shfl_sync(0xffffffffu, my_hi, 31);
         float m = -INFINITY, l = 0.f;
@@ -477,7 +475,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             __syncwarp();
             for (uint32_t again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
                 const int who = __ffs(again) - 1;
-                const int rr = half0 + (warp & 3) * 32 + who, ii = by_group(a, rr), hh = kh * a.group + rr - ii * a.group;
+                const int rr = half0 + (warp & 3) * 32 + who, ii = a.by_group.quotient(rr), hh = kh * a.group + rr - ii * a.group;
                 const int klo = __shfl_sync(0xffffffffu, in_lo, who), khi = __shfl_sync(0xffffffffu, in_hi, who);
                 const long long aa = (long long)(q0 + ii) * a.q_heads + hh;
                 const float2 ml = redo_row<T>(static_cast<const T *>(a.q) + (long long)(q0 + ii) * a.q_stride_row + hh * a.q_stride_head,
@@ -613,10 +611,7 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     const int wide = 1 << 30;  // beyond any sequence
     a.left = p->window_left < wide ? p->window_left : -1;
     a.right = p->window_right < wide ? p->window_right : -1;
-    int bits = 0;
-    while ((1LL << bits) < a.group) ++bits;
-    a.group_shift = (uint32_t)bits;
-    a.group_mul = (uint32_t)(((1ull << 32) * ((1ull << bits) - (unsigned)a.group)) / (unsigned)a.group + 1);
+    a.by_group = ofe::Divider((uint32_t)a.group);
     a.c = p->scale * 1.4426950408889634f;
     const int halves = halves_for(p);
     a.tiles = (int)(((long long)p->max_q * a.group + halves * kRows - 1) / (halves * kRows));

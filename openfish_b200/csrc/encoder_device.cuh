@@ -18,6 +18,18 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Division of numbers below 2^30 by a number that the host knows: a multiplication, an addition and a shift (the quotient is
+// exact: Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divider {
+    uint32_t mul, shift;
+    explicit Divider(uint32_t d = 1) {
+        shift = 0;
+        while ((1ull << shift) < d) ++shift;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int quotient(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+
 // Two 16-bit numbers in a register, and back.
 template <class T>
 __device__ __forceinline__ uint32_t pack(float a, float b);

@@ -45,16 +45,22 @@ struct Shape {
 
 struct Walk {  // the tiles in the order in which they are taken: stripes of 8 tiles of tokens, through all channels each
     int tiles_m, tiles_n;
+    ofe::Divider by_stripe, by_last;  // tiles of a stripe; tiles of tokens in the last one
+    Walk(int m, int n) : tiles_m(m), tiles_n(n), by_stripe((uint32_t)n * 8u), by_last((uint32_t)((m - 1) % 8 + 1)) {}
     __device__ __forceinline__ void at(int t, int *m, int *n) const {
-        const int stripe = t / (8 * tiles_n), first = stripe * 8;
-        const int high = min(8, tiles_m - first), in = t - stripe * 8 * tiles_n;
-        *m = first + in % high;
-        *n = in / high;
+        const int stripe = by_stripe.quotient(t), in = t - stripe * 8 * tiles_n;
+        if (stripe * 8 + 8 <= tiles_m) {
+            *n = in >> 3;
+            *m = stripe * 8 + (in & 7);
+        } else {
+            *n = by_last.quotient(in);
+            *m = stripe * 8 + in - *n * (tiles_m - stripe * 8);
+        }
     }
 };
 
 template <class T, int CG, int BN>
-__global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel(const Args a, const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel(const Args a, const Walk walk, const __grid_constant__ CUtensorMap map_x,
                                                                                  const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<CG, BN>;
     extern __shared__ uint8_t raw[];
@@ -69,7 +75,6 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 2 ? blockIdx.x & 1 : 0;
     const int group = blockIdx.x / CG, groups = gridDim.x / CG;
-    const Walk walk{(a.rows + 128 * CG - 1) / (128 * CG), (a.cols + BN - 1) / BN};
     const int tiles = walk.tiles_m * walk.tiles_n;
     const int steps = (a.depth + 127) / 128;
 
@@ -165,25 +170,24 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
         const T *const bias = static_cast<const T *>(a.bias);
         float2 next[S::kPart / 32];  // the next tile's scales and biases, a lane to a column
         float next_xs = 0.f;
+        int next_m0 = 0, next_n0 = 0;
         const auto fetch = [&](int t) {
             int tm, tn;
             walk.at(t, &tm, &tn);
-            const int m = tm * 128 * CG + rank * 128 + quarter * 32 + lane, n0 = tn * BN + part * S::kPart;
-            next_xs = t < tiles && m < a.rows ? a.x_scale[m] : 0.f;
+            next_m0 = tm * 128 * CG + rank * 128 + quarter * 32;
+            next_n0 = tn * BN + part * S::kPart;
+            next_xs = next_m0 + lane < a.rows ? a.x_scale[next_m0 + lane] : 0.f;
 #pragma unroll
             for (int i = 0; i < S::kPart / 32; ++i) {
-                const int n = n0 + i * 32 + lane;
-                const bool in = t < tiles && n < a.cols;
-                next[i].x = in ? a.w_scale[n] : 0.f;
-                next[i].y = in && bias ? ofe::to_float(bias[n]) : 0.f;
+                const int n = next_n0 + i * 32 + lane;
+                next[i].x = n < a.cols ? a.w_scale[n] : 0.f;
+                next[i].y = bias && n < a.cols ? ofe::to_float(bias[n]) : 0.f;
             }
         };
         fetch(group);
-        int j = 0, turn = 0;
+        int j = 0;
         for (int t = group; t < tiles; t += groups, ++j) {
-            int tm, tn;
-            walk.at(t, &tm, &tn);
-            const int m0 = tm * 128 * CG + rank * 128 + quarter * 32, n0 = tn * BN + part * S::kPart;
+            const int m0 = next_m0, n0 = next_n0;
             const float xs = next_xs;
             __syncwarp();  // the last tile's scales have been read
 #pragma unroll
@@ -192,11 +196,11 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                 biases[i * 32 + lane] = next[i].y;
             }
             __syncwarp();
-            fetch(t + groups);
+            if (t + groups < tiles) fetch(t + groups);
             if (!tc5::wait_warp(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status)) break;
             tc5::after_sync();
 #pragma unroll 1
-            for (int c = 0; c < S::kPart; c += 64, ++turn) {
+            for (int c = 0; c < S::kPart; c += 64) {
                 const uint32_t sum = tmem + ((uint32_t)(quarter * 32) << 16) + (j & 1) * BN + part * S::kPart + c;
                 uint32_t v[2][32];
                 tc5::ld64(v[0], v[1], sum);
@@ -279,7 +283,8 @@ int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
     if (!made) return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
     const auto kernel = matmul_tile_kernel<T, CG, BN>;
     if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
-    const long long tiles = ((long long)(a.rows + 128 * CG - 1) / (128 * CG)) * ((a.cols + BN - 1) / BN);
+    const Walk walk((a.rows + 128 * CG - 1) / (128 * CG), (a.cols + BN - 1) / BN);
+    const long long tiles = (long long)walk.tiles_m * walk.tiles_n;
     const int most = sms / CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
@@ -292,7 +297,7 @@ int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = CG > 1 ? 1 : 0;
-    return ofe::cuda_status(cudaLaunchKernelEx(&cfg, kernel, a, mx, mw, mo));
+    return ofe::cuda_status(cudaLaunchKernelEx(&cfg, kernel, a, walk, mx, mw, mo));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
