@@ -4,6 +4,7 @@
 //
 // A handful of tokens reads the weights once and is bound by that: matmul_few_kernel, four products to an
 // instruction.  Anything else goes to the matrix instructions: matmul_tile_kernel.
+#include <math.h>
 #include <stdint.h>
 
 #include "encoder_device.cuh"
@@ -301,62 +302,75 @@ int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// A few tokens: a warp to a channel, its lanes 16 bytes of the weights each at a time; the tokens come from the cache.
+// A few tokens: a warp to a channel, its lanes 16 bytes of the weights at a time; the tokens come from the cache.
 template <class T, int MT>
 __global__ void __launch_bounds__(128) matmul_few_kernel(const Args a) {
     const int lane = threadIdx.x & 31;
-    const int n = blockIdx.x * 4 + (threadIdx.x >> 5), m0 = blockIdx.y * MT;
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (n >= a.cols) return;
-    int sum[MT] = {};
     const int8_t *const w = a.w + (long long)n * a.w_stride;
-#pragma unroll 4
-    for (int k = lane * 16; k < a.depth; k += 512) {
-        int4 wv = *reinterpret_cast<const int4 *>(w + k);
-        if (k + 16 > a.depth) {  // what lies behind the row is no part of it
+    const int8_t *x[MT];  // (tokens that are not there: the last one again)
+    int sum[MT] = {};
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = a.x + min(i, a.rows - 1) * a.x_stride;
+    const auto add = [&](int k, int keep) {  // 16 of the depth, `keep` of them in it
+        int4 wv = *reinterpret_cast<const int4 *>(w + k), xv[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xv[i] = *reinterpret_cast<const int4 *>(x[i] + k);
+        if (keep < 16) {
             int *const word = reinterpret_cast<int *>(&wv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int keep = a.depth - k - 4 * i;  // bytes of this word
-                word[i] = keep >= 4 ? word[i] : keep <= 0 ? 0 : word[i] & ((1 << (8 * keep)) - 1);
+            for (int b = 0; b < 4; ++b) {
+                const int left = keep - 4 * b;  // bytes of this word
+                word[b] = left >= 4 ? word[b] : left <= 0 ? 0 : word[b] & ((1 << (8 * left)) - 1);
             }
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            if (m0 + i < a.rows) {
-                const int4 xv = *reinterpret_cast<const int4 *>(a.x + (m0 + i) * a.x_stride + k);
-                sum[i] = __dp4a(xv.x, wv.x, sum[i]);
-                sum[i] = __dp4a(xv.y, wv.y, sum[i]);
-                sum[i] = __dp4a(xv.z, wv.z, sum[i]);
-                sum[i] = __dp4a(xv.w, wv.w, sum[i]);
-            }
+            sum[i] = __dp4a(xv[i].x, wv.x, sum[i]);
+            sum[i] = __dp4a(xv[i].y, wv.y, sum[i]);
+            sum[i] = __dp4a(xv[i].z, wv.z, sum[i]);
+            sum[i] = __dp4a(xv[i].w, wv.w, sum[i]);
         }
-    }
+    };
+    int k = lane * 16;
+#pragma unroll 4
+    for (; k + 16 <= a.depth; k += 512) add(k, 16);
+    if (k < a.depth) add(k, a.depth - k);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int s = __reduce_add_sync(0xffffffffu, sum[i]);
-        if (lane == i && m0 + i < a.rows) {
+        if (lane == i && i < a.rows) {
             const float b = a.bias ? ofe::to_float(static_cast<const T *>(a.bias)[n]) : 0.f;
-            static_cast<T *>(a.out)[(m0 + i) * a.out_stride + n] = ofe::from_float<T>(fmaf((float)s, a.x_scale[m0 + i] * a.w_scale[n], b));
+            static_cast<T *>(a.out)[i * a.out_stride + n] = ofe::from_float<T>(fmaf((float)s * a.x_scale[i], a.w_scale[n], b));
         }
     }
 }
 
 template <class T, int MT>
 int launch_few(const Args &a, cudaStream_t stream) {
-    matmul_few_kernel<T, MT><<<dim3((unsigned)((a.cols + 3) / 4), (unsigned)((a.rows + MT - 1) / MT)), 128, 0, stream>>>(a);
+    matmul_few_kernel<T, MT><<<(unsigned)((a.cols + 3) / 4), 128, 0, stream>>>(a);
     return ofe::launched();
 }
 
+// Up to 8 tokens go to the dot products: us for 1, 4 and 8 tokens there / by the smallest tiles, 4096 x 4096: 3.4, 4.8, 7.5 / 14; 8192 x 1024: 2.7,
+// 4.5, 6.5 / 6.7; 512 x 512: 1.6, 2.1, 2.6 / 3.9.
+// Of the tiles, those whose rounds over the SMs are estimated to end first: a start, and a time for every 128 of the depth of a
+// round.  Measured (us by 64, 128, 256 wide tiles, the chosen one first): 512 x 1536 x 512 4.3, 4.8, 6.6; 512 x 8192 x 1024 8.0 (256), 8.5, 11.8; 1003 x 2504 x
+// 1237 8.8 (256), 10.3, 11.0; 2048 x 1536 x 512 6.2 (128), 6.7, 6.8; 4096 x 4096 x 4096 45 (256), 62, 109.
 template <class T>
 int run(const Args &a, int sms, cudaStream_t stream) {
     if (a.rows <= 1) return launch_few<T, 1>(a, stream);
     if (a.rows <= 2) return launch_few<T, 2>(a, stream);
     if (a.rows <= 4) return launch_few<T, 4>(a, stream);
     if (a.rows <= 8) return launch_few<T, 8>(a, stream);
-    const long long tiles_m = (a.rows + 127) / 128;
-    if (tiles_m * ((a.cols + 127) / 128) <= sms) return launch_tiles<T, 1, 64>(a, sms, stream);
-    if (((tiles_m + 1) / 2) * ((a.cols + 255) / 256) * 2 <= sms) return launch_tiles<T, 1, 128>(a, sms, stream);
-    return launch_tiles<T, 2, 256>(a, sms, stream);
+    const auto estimate = [&](int high, int wide, int at_once, double start, double step) {
+        const double tiles = (double)((a.rows + high - 1) / high) * ((a.cols + wide - 1) / wide);
+        return start + ceil(tiles / at_once) * ((a.depth + 127) / 128) * step;
+    };
+    const double t64 = estimate(128, 64, sms, 3.0, 0.25), t128 = estimate(128, 128, sms, 3.6, 0.30), t256 = estimate(256, 256, sms / 2, 5.4, 0.36);
+    if (t64 <= t128 && t64 <= t256) return launch_tiles<T, 1, 64>(a, sms, stream);
+    return t128 < t256 ? launch_tiles<T, 1, 128>(a, sms, stream) : launch_tiles<T, 2, 256>(a, sms, stream);
 }
 
 }  // namespace
