@@ -77,9 +77,13 @@ __device__ __forceinline__ float reduce(float v, float *scratch, Op op) {
 }
 
 // BLOCK: a block to a row, else a warp.  CH packs of V elements to a thread.
-template <class T, int V, int CH, bool BLOCK>
+// SHIFT: rows that start anywhere, all tensors' in the same place between two 16-byte boundaries.  The packs are the aligned 16 bytes
+// around the row, and which thread has which element does not matter to a sum: elements of a pack that lie in front of the row or
+// behind it are taken as zeros and not written.
+template <class T, int V, int CH, bool BLOCK, bool SHIFT>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs<T> a) {
     __shared__ float scratch[32];
+    constexpr int P = (V + 1) / 2;
     const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
     const int lanes = BLOCK ? blockDim.x : 32;
     const long long step = BLOCK ? gridDim.x : (long long)gridDim.x * (blockDim.x >> 5);
@@ -88,28 +92,52 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
     const auto most = [](float p, float q) { return fmaxf(p, q); };
     const float inv = 1.f / (float)a.width;
 
-    constexpr int P = (V + 1) / 2;
     for (long long row = first; row < a.rows; row += step) {
         const T *const x = a.x + row * a.x_stride, *const r = a.r + row * a.r_stride;
+        const int shift = SHIFT ? (int)((uintptr_t)x & 15) / 2 : 0;
+        const auto place = [&](int c) { return (c * lanes + lane) * V - shift; };            // a pack's first element
+        const auto here = [&](int at) { return at < a.width && (!SHIFT || at > -V); };        // whether it has any of the row
+        const auto whole = [&](int at) { return !SHIFT || (at >= 0 && at + V <= a.width); };  // or nothing else
+        const auto trim = [&](int at, float2 (&f)[P]) {  // nothing but the row's elements
+            if (whole(at)) return;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (at + 2 * i < 0 || at + 2 * i >= a.width) f[i].x = 0.f;
+                if (at + 2 * i + 1 < 0 || at + 2 * i + 1 >= a.width) f[i].y = 0.f;
+            }
+        };
+        const auto along = [&](const T *p, int at, float2 (&f)[P]) {  // a weight or bias
+            if (!SHIFT) {
+                read<T, V>(p + at, f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i) f[i] = make_float2(to_float(p[min(max(at + 2 * i, 0), a.width - 1)]), to_float(p[min(max(at + 2 * i + 1, 0), a.width - 1)]));
+            }
+        };
         float2 s[CH][P];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = (c * lanes + lane) * V;
+            const int at = place(c);
 #pragma unroll
             for (int i = 0; i < P; ++i) s[c][i] = {0.f, 0.f};
-            if (at < a.width) read<T, V>(x + at, s[c]);
+            if (here(at)) read<T, V>(x + at, s[c]);
         }
         if (a.r) {
             float2 f[CH][P];
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int at = (c * lanes + lane) * V;
-                if (at < a.width) {
+                const int at = place(c);
+                if (here(at)) {
                     read<T, V>(r + at, f[c]);
 #pragma unroll
                     for (int i = 0; i < P; ++i) s[c][i] = fma2(f[c][i], {a.alpha, a.alpha}, s[c][i]);
                 }
             }
+        }
+        if (SHIFT) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                if (here(place(c))) trim(place(c), s[c]);
         }
         if (a.kind != OPENFISH_B200_NORM_NONE) {
             float2 sum = {0.f, 0.f};
@@ -122,9 +150,11 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
                 sum = {0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    if ((c * lanes + lane) * V < a.width) {
+                    const int at = place(c);
+                    if (here(at)) {
 #pragma unroll
                         for (int i = 0; i < P; ++i) s[c][i] = add2(s[c][i], {-mean, V == 1 ? 0.f : -mean});
+                        trim(at, s[c]);
                     }
                 }
             }
@@ -135,29 +165,38 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
             const float factor = 1.f / sqrtf(reduce<BLOCK>(sum.x + sum.y, scratch, add) * inv + a.eps);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int at = (c * lanes + lane) * V;
-                if (at < a.width) {
+                const int at = place(c);
+                if (here(at)) {
                     float2 f[P];
 #pragma unroll
                     for (int i = 0; i < P; ++i) s[c][i] = mul2(s[c][i], {factor, factor});
                     if (a.w) {
-                        read<T, V>(a.w + at, f);
+                        along(a.w, at, f);
 #pragma unroll
                         for (int i = 0; i < P; ++i) s[c][i] = mul2(s[c][i], f[i]);
                     }
                     if (a.b) {
-                        read<T, V>(a.b + at, f);
+                        along(a.b, at, f);
 #pragma unroll
                         for (int i = 0; i < P; ++i) s[c][i] = add2(s[c][i], f[i]);
                     }
+                    trim(at, s[c]);
                 }
             }
         }
         if (a.out) {
+            T *const out = a.out + row * a.out_stride;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int at = (c * lanes + lane) * V;
-                if (at < a.width) write<T, V>(a.out + row * a.out_stride + at, s[c]);
+                const int at = place(c);
+                if (!here(at)) continue;
+                if (whole(at)) {
+                    write<T, V>(out + at, s[c]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (at + i >= 0 && at + i < a.width) out[at + i] = from_float<T>(i & 1 ? s[c][i / 2].y : s[c][i / 2].x);
+                }
             }
         }
         if (!a.q) continue;
@@ -174,48 +213,53 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
         const bool fine = top < INFINITY;
         const float back = 127.f / top;  // no number for a row of zeros, and beyond fp32 for one whose top is below 2^-121
         const bool direct = back < INFINITY;
+        int8_t *const q = a.q + row * a.q_stride;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = (c * lanes + lane) * V;
-            if (at < a.width) {
-                alignas(8) int8_t o[V];
+            const int at = place(c);
+            if (!here(at)) continue;
+            alignas(8) int8_t o[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float y = i & 1 ? s[c][i / 2].y : s[c][i / 2].x;
-                    const float f = direct ? y * back : top > 0.f ? y / top * 127.f : 0.f;
-                    // (|f| is at most 127 and a rounding: no clamp can be reached)
-                    o[i] = fine ? (int8_t)__float2int_rn(f) : (int8_t)0;
-                }
-                if (V == 8) *reinterpret_cast<uint2 *>(a.q + row * a.q_stride + at) = *reinterpret_cast<const uint2 *>(o);
-                else a.q[row * a.q_stride + at] = o[0];
+            for (int i = 0; i < V; ++i) {
+                const float y = i & 1 ? s[c][i / 2].y : s[c][i / 2].x;
+                const float f = direct ? y * back : top > 0.f ? y / top * 127.f : 0.f;
+                // (|f| is at most 127 and a rounding: no clamp can be reached)
+                o[i] = fine ? (int8_t)__float2int_rn(f) : (int8_t)0;
+            }
+            if (V == 8 && !SHIFT) {
+                *reinterpret_cast<uint2 *>(q + at) = *reinterpret_cast<const uint2 *>(o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (!SHIFT || (at + i >= 0 && at + i < a.width)) q[at + i] = o[i];
             }
         }
         if (lane == 0) a.q_scale[row] = fine ? top / 127.f : NAN;
     }
 }
 
-template <class T, int V, int CH, bool BLOCK>
+template <class T, int V, int CH, bool BLOCK, bool SHIFT>
 void launch(const NormArgs<T> &a, int threads, int sms, cudaStream_t stream) {
     const long long per_block = BLOCK ? 1 : threads / 32;
     long long blocks = (a.rows + per_block - 1) / per_block;
-    // Up to 32 warps to a scheduler's worth of rows in turn (53312 rows of 512 with a residual, us by blocks of full occupancy: one 32.2, two 31.1,
-    // four 32.0, a block to four rows 32.8).
+    // Rows in turn for two blocks where one fits (53312 rows of 512 with a residual, us with one, two, four blocks: 32.2,
+    // 31.1, 32.0; with a block to every four rows 32.8).
     const long long cap = (long long)sms * (2048 / threads) * 2;
     if (blocks > cap) blocks = cap;
-    norm_kernel<T, V, CH, BLOCK><<<(unsigned)blocks, threads, 0, stream>>>(a);
+    norm_kernel<T, V, CH, BLOCK, SHIFT><<<(unsigned)blocks, threads, 0, stream>>>(a);
 }
 
 // A warp to a row while 4 packs (of one element: 16) to a lane hold it, else a block with as few packs to a thread as 1024
 // threads allow.
-template <class T, int V>
+template <class T, int V, bool SHIFT>
 void dispatch(const NormArgs<T> &a, int sms, cudaStream_t stream) {
-    const int packs = (a.width + V - 1) / V;
-    constexpr int S = V == 8 ? 1 : 4;  // scalar packs are an eighth of the size: more of them
-    if (packs <= 32 * S) launch<T, V, S, false>(a, 128, sms, stream);
-    else if (packs <= 64 * S) launch<T, V, 2 * S, false>(a, 128, sms, stream);
-    else if (packs <= 128 * S) launch<T, V, 4 * S, false>(a, 128, sms, stream);
-    else if (packs <= 1024 * S) launch<T, V, S, true>(a, ((packs + S - 1) / S + 31) / 32 * 32, sms, stream);
-    else launch<T, V, 4 * (8 / V), true>(a, 1024, sms, stream);
+    const int packs = (a.width + V - 1) / V + SHIFT;
+    constexpr int S = V == 8 ? 1 : 4;  // single elements are an eighth of a pack: more of them
+    if (packs <= 32 * S) launch<T, V, S, false, SHIFT>(a, 128, sms, stream);
+    else if (packs <= 64 * S) launch<T, V, 2 * S, false, SHIFT>(a, 128, sms, stream);
+    else if (packs <= 128 * S) launch<T, V, 4 * S, false, SHIFT>(a, 128, sms, stream);
+    else if (packs <= 1024 * S) launch<T, V, S, true, SHIFT>(a, ((packs + S - 1) / S + 31) / 32 * 32, sms, stream);
+    else launch<T, V, 4 * (8 / V) + SHIFT, true, SHIFT>(a, 1024, sms, stream);
 }
 
 template <class T>
@@ -229,11 +273,17 @@ int run(cudaStream_t stream, const openfish_b200_norm_t *p, int sms) {
     const auto fits = [&](const void *q, long long stride, int to) {
         return !q || ((uintptr_t)q % to == 0 && (p->rows == 1 || stride % 8 == 0));
     };
+    // a tensor whose rows all start where x's do between two 16-byte boundaries
+    const auto beside = [&](const void *q, long long stride) {
+        return !q || (((uintptr_t)q ^ (uintptr_t)p->x) % 16 == 0 && (p->rows == 1 || (stride - p->x_stride) % 8 == 0));
+    };
     if (p->width % 8 == 0 && fits(p->x, p->x_stride, 16) && fits(p->residual, p->residual_stride, 16) && fits(p->weight, 0, 16) &&
         fits(p->bias, 0, 16) && fits(p->out, p->out_stride, 16) && fits(p->q, p->q_stride, 8))
-        dispatch<T, 8>(a, sms, stream);
+        dispatch<T, 8, false>(a, sms, stream);
+    else if (beside(p->residual, p->residual_stride) && beside(p->out, p->out_stride))
+        dispatch<T, 8, true>(a, sms, stream);
     else
-        dispatch<T, 1>(a, sms, stream);
+        dispatch<T, 1, false>(a, sms, stream);
     return ofe::launched();
 }
 

@@ -72,6 +72,20 @@ def test_strides_and_offsets(native_lib, dtype, width):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1, 3, 7, 9, 15, 101, 250, 511, 1021, 1023, 2001, 4099, 8191, 8193, 32767])
+@pytest.mark.parametrize("kind", ["layer", "rms", "none"])
+def test_odd_widths_next_to_rows_that_hold_no_numbers(native_lib, dtype, width, kind):
+    # rows without room between them: what is read around a row is its neighbours', and has no part in it
+    x, r = make(9, width, dtype, 1), make(9, width, dtype, 2)
+    w, b = (None, None) if kind == "none" else (make(1, width, dtype, 3, 0.2, 1.0)[0], make(1, width, dtype, 4)[0])
+    clean, q, scale = check(native_lib, x, kind, w, b, residual=r, residual_scale=0.5)
+    x[::2], r[::2] = math.nan, math.inf
+    got, q2, scale2 = native_lib.norm(x, kind, w, b, residual=r, residual_scale=0.5, quantize=True)
+    assert torch.equal(got[1::2], clean[1::2]) and torch.equal(q[1::2], q2[1::2]) and torch.equal(scale[1::2], scale2[1::2])
+    assert torch.isnan(scale2[::2]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("width", [96, 101, 6000])
 def test_in_place(native_lib, dtype, width):
     x, r = make(50, width, dtype, 1), make(50, width, dtype, 2)
