@@ -267,8 +267,8 @@ void openfish_b200_matmul_i8(void *cuda_stream, const openfish_b200_matmul_i8_t 
  * weight and bias [width] or NULL (1 and 0; kind NONE takes neither).  out (or NULL): y in the type of x.  q (or NULL): y in
  * 8 bits, q = round(y * 127 / top) to nearest, ties to even, and q_scale[row] = top / 127 with top = max |y| of the row (from the unrounded y); a row of zeros gets
  * zeros and scale 0, a row with an infinity or NaN zeros and scale NaN.  width up to 32768.  out may be x or
- * residual themselves (same pointer, same stride).  Rows of x and residual may be read up to the 16-byte boundaries around them, what
- * lies there is not used. */
+ * residual themselves (same pointer, same stride).  Rows of x and residual, weight and bias may be read up to the 16-byte boundaries around them,
+ * what lies there is not used. */
 enum openfish_b200_norm_kind { OPENFISH_B200_NORM_NONE = 0, OPENFISH_B200_NORM_LAYER = 1, OPENFISH_B200_NORM_RMS = 2 };
 typedef struct openfish_b200_norm {
     int dtype; /* of x, residual, weight, bias and out */

@@ -32,6 +32,7 @@ struct NormArgs {
     long long x_stride, r_stride, out_stride, q_stride, rows;
     int width, kind;
     float eps, alpha;
+    bool w_packs, q_packs;  // weight and bias, the codes' rows: on boundaries of a pack, whatever the rows of x are on
 };
 
 // V elements that lie together, two at a time: 16 bytes where everything is aligned to that, else one element (and a
@@ -109,6 +110,19 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
         const auto along = [&](const T *p, int at, float2 (&f)[P]) {  // a weight or bias
             if (!SHIFT) {
                 read<T, V>(p + at, f);
+            } else if (a.w_packs) {
+                // the two packs that the eight lie in, moved by n elements (the same n in the whole row)
+                const int n = at & 7, k = at - n;
+                uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+                if (k >= 0 && k < a.width) v0 = *reinterpret_cast<const uint4 *>(p + k);
+                if (n > 0 && k + 8 < a.width) v1 = *reinterpret_cast<const uint4 *>(p + k + 8);
+                uint32_t m[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                for (int i = 0; i < 6; ++i) m[i] = n & 4 ? m[i + 2] : m[i];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) m[i] = n & 2 ? m[i + 1] : m[i];
+#pragma unroll
+                for (int i = 0; i < P; ++i) f[i] = ofe::unpack<T>(n & 1 ? __byte_perm(m[i], m[i + 1], 0x5432) : m[i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < P; ++i) f[i] = make_float2(to_float(p[min(max(at + 2 * i, 0), a.width - 1)]), to_float(p[min(max(at + 2 * i + 1, 0), a.width - 1)]));
@@ -214,24 +228,49 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
         const float back = 127.f / top;  // no number for a row of zeros, and beyond fp32 for one whose top is below 2^-121
         const bool direct = back < INFINITY;
         int8_t *const q = a.q + row * a.q_stride;
+        uint64_t codes[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const int at = place(c);
-            if (!here(at)) continue;
-            alignas(8) int8_t o[V];
+            alignas(8) int8_t o[8];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < 8; ++i) {
+                if (i >= V) break;
                 const float y = i & 1 ? s[c][i / 2].y : s[c][i / 2].x;
                 const float f = direct ? y * back : top > 0.f ? y / top * 127.f : 0.f;
                 // (|f| is at most 127 and a rounding: no clamp can be reached)
                 o[i] = fine ? (int8_t)__float2int_rn(f) : (int8_t)0;
             }
+            if (V == 8) codes[c] = *reinterpret_cast<const uint64_t *>(o);
+            else codes[c] = (uint8_t)o[0];
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = place(c);
             if (V == 8 && !SHIFT) {
-                *reinterpret_cast<uint2 *>(q + at) = *reinterpret_cast<const uint2 *>(o);
-            } else {
+                if (here(at)) *reinterpret_cast<uint64_t *>(q + at) = codes[c];
+            } else if (V == 8 && a.q_packs) {
+                // the eight codes from the next boundary on: the end of these and the beginning of the next thread's (of the last
+                // thread in a warp: of the first one's next pack; in a block that is another warp, and the codes go one by one)
+                uint64_t after = __shfl_down_sync(0xffffffffu, codes[c], 1);
+                const int in_warp = lane & 31, to = at + shift;
+                if (!BLOCK && CH > 1) {
+                    const uint64_t first_next = __shfl_sync(0xffffffffu, codes[c + 1 < CH ? c + 1 : c], 0);
+                    if (in_warp == 31) after = first_next;
+                }
+                const uint64_t both = shift == 0 ? codes[c] : codes[c] >> (8 * shift) | after << (64 - 8 * shift);
+                const int mine = BLOCK && in_warp == 31 ? 8 - shift : 8;
+                if (mine == 8 && to + 8 <= a.width) {
+                    *reinterpret_cast<uint64_t *>(q + to) = both;
+                } else {
+                    for (int i = 0; i < mine && to + i < a.width; ++i) q[to + i] = (int8_t)(both >> (8 * i));
+                }
+                if (BLOCK && in_warp == 0)
+                    for (int i = 0; i < shift; ++i)
+                        if (at + i >= 0 && at + i < a.width) q[at + i] = (int8_t)(codes[c] >> (8 * i));
+            } else if (here(at)) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (!SHIFT || (at + i >= 0 && at + i < a.width)) q[at + i] = o[i];
+                    if (!SHIFT || (at + i >= 0 && at + i < a.width)) q[at + i] = (int8_t)(codes[c] >> (8 * i));
             }
         }
         if (lane == 0) a.q_scale[row] = fine ? top / 127.f : NAN;
@@ -257,6 +296,7 @@ void dispatch(const NormArgs<T> &a, int sms, cudaStream_t stream) {
     constexpr int S = V == 8 ? 1 : 4;  // single elements are an eighth of a pack: more of them
     if (packs <= 32 * S) launch<T, V, S, false, SHIFT>(a, 128, sms, stream);
     else if (packs <= 64 * S) launch<T, V, 2 * S, false, SHIFT>(a, 128, sms, stream);
+    else if (packs <= 96 * S) launch<T, V, 3 * S, false, SHIFT>(a, 128, sms, stream);
     else if (packs <= 128 * S) launch<T, V, 4 * S, false, SHIFT>(a, 128, sms, stream);
     else if (packs <= 1024 * S) launch<T, V, S, true, SHIFT>(a, ((packs + S - 1) / S + 31) / 32 * 32, sms, stream);
     else launch<T, V, 4 * (8 / V) + SHIFT, true, SHIFT>(a, 1024, sms, stream);
@@ -269,6 +309,8 @@ int run(cudaStream_t stream, const openfish_b200_norm_t *p, int sms) {
     a.w = static_cast<const T *>(p->weight); a.b = static_cast<const T *>(p->bias);
     a.out = static_cast<T *>(p->out); a.q = p->q; a.q_scale = p->q_scale;
     a.x_stride = p->x_stride; a.r_stride = p->residual_stride; a.out_stride = p->out_stride; a.q_stride = p->q_stride;
+    a.w_packs = ((uintptr_t)p->weight | (uintptr_t)p->bias) % 16 == 0;
+    a.q_packs = (uintptr_t)p->q % 8 == 0 && (p->rows == 1 || p->q_stride % 8 == 0);
     a.rows = p->rows; a.width = p->width; a.kind = p->kind; a.eps = p->eps; a.alpha = p->residual_scale;
     const auto fits = [&](const void *q, long long stride, int to) {
         return !q || ((uintptr_t)q % to == 0 && (p->rows == 1 || stride % 8 == 0));
