@@ -46,6 +46,7 @@ struct Args {
     ofe::Divider by_group;
     int tiles, splits;  // blocks of rows to the longest sequence; pieces of a block's keys
     float c;
+    bool q_by_copy;  // the group divides a half's rows: a tiled copy brings the queries
 };
 
 // A sequence's rows in a tensor of `rows`, cut to the room there is.
@@ -142,7 +143,8 @@ __device__ __noinline__ float2 redo_row(const T *q, const T *k, const T *v, long
 }
 
 template <class T, int DP, int H>
-__global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_q,
+                                                                                                  const __grid_constant__ CUtensorMap map_k,
                                                                                                   const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<DP, H>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -206,11 +208,24 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
         }
         for (int i = 0; i < H; ++i) ofd::mbar_init(&my_turn[i], 1);
         for (int i = 0; i < H * S::kHalfBarriers; ++i) {
-            // s_full and o_done are a commit's, p_ready and q_ready take an arrival of each warp
+            // s_full and o_done are a commit's, p_ready takes an arrival of each warp, and so does q_ready without a copy
             const int of = i % S::kHalfBarriers;
-            ofd::mbar_init(&of_half[i], of < S::kBuffers || of > 2 * S::kBuffers ? 1 : 4);
+            ofd::mbar_init(&of_half[i], of < S::kBuffers || of > 2 * S::kBuffers || (of == 2 * S::kBuffers && a.q_by_copy) ? 1 : 4);
         }
         ofd::mbar_fence_init();
+        if (a.q_by_copy) {
+            // rows that are not there come as whatever lies behind the sequence: each row of a product is by itself
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                if (to[i] <= from[i]) continue;
+                uint64_t *const bar = of_half + i * S::kHalfBarriers + 2 * S::kBuffers;
+                ofd::mbar_arrive_expect_tx(bar, S::kQueryBytes);
+#pragma unroll
+                for (int d = 0; d < S::kChunks; ++d)
+                    tc5::load_3d(q_tiles + i * S::kQueryBytes + d * kRows * 128, &map_q, d * 64, kh * a.group,
+                                 q0 + a.by_group.quotient(r0 + i * kRows), bar);
+            }
+        }
         for (int i = 0; i < S::kStages && i < steps; ++i) load(i, i);
     }
     if (warp == 4 * H) tc5::tmem_alloc<1>(tmem_slot, S::kColumns);
@@ -307,7 +322,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
         const int r = half0 + row, i = a.by_group.quotient(r), head = kh * a.group + r - i * a.group;
         const bool there = r < rows, warp_there = half0 + (warp & 3) * 32 < rows;
         // ---- the queries into shared memory, pieces of 16 bytes; zeros where there are none
-        if (end > begin) {
+        if (end > begin && !a.q_by_copy) {
             constexpr int kPieces = DP / 8;
 #pragma unroll 4
             for (int n = threadIdx.x & 127; n < kRows * kPieces; n += 128) {
@@ -556,20 +571,22 @@ int splits_for(const openfish_b200_attention_t *a, int sms) {
     return n < 1 ? 1 : (int)n;
 }
 
-bool heads_map(CUtensorMap *map, bool bf16, const void *base, const openfish_b200_attention_t *a, long long stride_row, long long stride_head) {
-    const cuuint64_t dims[3] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->kv_heads, (cuuint64_t)a->k_rows};
-    const cuuint64_t strides[2] = {(cuuint64_t)(a->kv_heads > 1 ? stride_head : 128) * 2, (cuuint64_t)(a->k_rows > 1 ? stride_row : 128) * 2};
-    const cuuint32_t box[3] = {64, 1, kKeys};
+// [rows][heads][head_dim] in boxes of 64 elements, `box_heads` heads and `box_rows` rows.
+bool heads_map(CUtensorMap *map, bool bf16, const void *base, int head_dim, int heads, long long rows, long long stride_row, long long stride_head,
+               int box_heads, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? stride_head : 128) * 2, (cuuint64_t)(rows > 1 ? stride_row : 128) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
     return tc5::make_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box);
 }
 
 template <class T, int DP, int H>
-int launch(const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
+int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
     using S = Shape<DP, H>;
     const auto kernel = attention_kernel<T, DP, H>;
     if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
     const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
-    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mk, mv);
+    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mq, mk, mv);
     if (const int rc = ofe::launched()) return rc;
     if (a.splits == 1) return OPENFISH_B200_OK;
     const long long joins = ((long long)a.max_q * a.q_heads * a.sequences + 3) / 4;
@@ -578,9 +595,9 @@ int launch(const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStre
 }
 
 template <class T>
-int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, int halves, cudaStream_t stream) {
-    if (p->head_dim <= 64) return launch<T, 64, 1>(a, mk, mv, stream);
-    return halves == 1 ? launch<T, 128, 1>(a, mk, mv, stream) : launch<T, 128, 2>(a, mk, mv, stream);
+int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, int halves, cudaStream_t stream) {
+    if (p->head_dim <= 64) return launch<T, 64, 1>(a, mq, mk, mv, stream);
+    return halves == 1 ? launch<T, 128, 1>(a, mq, mk, mv, stream) : launch<T, 128, 2>(a, mq, mk, mv, stream);
 }
 
 size_t part_bytes(const openfish_b200_attention_t *a, int splits) {
@@ -624,16 +641,17 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
         a.part_lse = a.part + (size_t)a.splits * a.q_rows * a.q_heads * a.head_dim;
     }
     const bool bf16 = p->dtype == OPENFISH_B200_BF16;
-    CUtensorMap mk, mv;
-    openfish_b200_attention_t none = *p;  // no keys at all: the kernel copies nothing, but a map has to be one of something
-    const void *k = p->k, *v = p->v;
-    if (p->k_rows == 0) {
-        none.k_rows = none.kv_heads = 1;
-        k = v = p->q;
-    }
-    if (!heads_map(&mk, bf16, k, &none, p->k_stride_row, p->k_stride_head) || !heads_map(&mv, bf16, v, &none, p->v_stride_row, p->v_stride_head))
-        return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
-    return bf16 ? launch_for<__nv_bfloat16>(p, a, mk, mv, halves, (cudaStream_t)stream) : launch_for<__half>(p, a, mk, mv, halves, (cudaStream_t)stream);
+    CUtensorMap mq, mk, mv;
+    const int d = p->head_dim, hk = p->kv_heads;
+    bool made = p->k_rows == 0  // no keys at all: the kernel copies nothing, but a map has to be one of something
+                    ? heads_map(&mk, bf16, p->q, d, 1, 1, 0, 0, 1, kKeys) && heads_map(&mv, bf16, p->q, d, 1, 1, 0, 0, 1, kKeys)
+                    : heads_map(&mk, bf16, p->k, d, hk, p->k_rows, p->k_stride_row, p->k_stride_head, 1, kKeys) &&
+                          heads_map(&mv, bf16, p->v, d, hk, p->k_rows, p->v_stride_row, p->v_stride_head, 1, kKeys);
+    a.q_by_copy = kRows % a.group == 0;
+    mq = mk;
+    if (a.q_by_copy) made = made && heads_map(&mq, bf16, p->q, d, p->q_heads, p->q_rows, p->q_stride_row, p->q_stride_head, a.group, kRows / a.group);
+    if (!made) return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
+    return bf16 ? launch_for<__nv_bfloat16>(p, a, mq, mk, mv, halves, (cudaStream_t)stream) : launch_for<__half>(p, a, mq, mk, mv, halves, (cudaStream_t)stream);
 }
 
 extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }
