@@ -46,7 +46,8 @@ struct Args {
     ofe::Divider by_group;
     int tiles, splits;  // blocks of rows to the longest sequence; pieces of a block's keys
     float c;
-    bool q_by_copy;  // the group divides a half's rows: a tiled copy brings the queries
+    bool q_by_copy;    // the group divides a half's rows: a tiled copy brings the queries
+    bool out_by_copy;  // it divides a warp's rows: and takes the results
 };
 
 // A sequence's rows in a tensor of `rows`, cut to the room there is.
@@ -145,7 +146,8 @@ __device__ __noinline__ float2 redo_row(const T *q, const T *k, const T *v, long
 template <class T, int DP, int H>
 __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks) attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_q,
                                                                                                   const __grid_constant__ CUtensorMap map_k,
-                                                                                                  const __grid_constant__ CUtensorMap map_v) {
+                                                                                                  const __grid_constant__ CUtensorMap map_v,
+                                                                                                  const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<DP, H>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -461,13 +463,15 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             T *const out = static_cast<T *>(a.out) + (long long)(q0 + i) * a.out_stride_row + head * a.out_stride_head;
             float *const part = a.part + ((long long)split * a.q_rows * a.q_heads + at) * a.head_dim;
             bool bad = false;
+            // A warp whose rows are all there puts them where its queries were, and a tiled copy takes them out; else each thread
+            // writes its own.
+            const bool by_copy = a.out_by_copy && a.splits == 1 && half0 + (warp & 3) * 32 + 32 <= rows;
+            uint8_t *const staged = q_tile + (warp & 3) * 4096;
 #pragma unroll 1
             for (int n = 0; n < DP; n += 32) {
                 uint32_t o[32];
                 __syncwarp();
-                if (any) {
-                    tc5::ld32(o, o_at + n);
-                }
+                if (any) tc5::ld32(o, o_at + n);
                 if (!there) continue;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
@@ -478,12 +482,34 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                         f[b] = sees ? __uint_as_float(o[e + b]) * back : 0.f;
                         bad |= !(fabsf(f[b]) < INFINITY);
                     }
-                    if (a.splits == 1) {
-                        *reinterpret_cast<uint4 *>(out + n + e) = make_uint4(pack<T>(f[0], f[1]), pack<T>(f[2], f[3]), pack<T>(f[4], f[5]), pack<T>(f[6], f[7]));
+                    const uint4 packed = make_uint4(pack<T>(f[0], f[1]), pack<T>(f[2], f[3]), pack<T>(f[4], f[5]), pack<T>(f[6], f[7]));
+                    if (by_copy) {
+                        *reinterpret_cast<uint4 *>(staged + ((n + e) >> 6) * kRows * 128 + lane * 128 + ((((n + e) >> 3 & 7) ^ (lane & 7)) << 4)) = packed;
+                    } else if (a.splits == 1) {
+                        *reinterpret_cast<uint4 *>(out + n + e) = packed;
                     } else {
                         *reinterpret_cast<float4 *>(part + n + e) = make_float4(f[0], f[1], f[2], f[3]);
                         *reinterpret_cast<float4 *>(part + n + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
                     }
+                }
+            }
+            if (by_copy) {
+                if (!__any_sync(0xffffffffu, bad)) {
+                    tc5::fence_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int first_row = half0 + (warp & 3) * 32, token = a.by_group.quotient(first_row);
+#pragma unroll
+                        for (int d = 0; d < S::kChunks; ++d)
+                            if (d * 64 < a.head_dim)
+                                tc5::store_3d(&map_out, d * 64, kh * a.group + first_row - token * a.group, q0 + token, staged + d * kRows * 128);
+                        tc5::store_commit();
+                        tc5::store_wait_read<0>();
+                    }
+                } else {  // (the rows that are done again must not meet a copy that is under way)
+                    for (int n = 0; n < a.head_dim; n += 8)
+                        *reinterpret_cast<uint4 *>(out + n) =
+                            *reinterpret_cast<const uint4 *>(staged + (n >> 6) * kRows * 128 + lane * 128 + (((n >> 3 & 7) ^ (lane & 7)) << 4));
                 }
             }
             float lse = sees ? m * a.c + log2f(l) : -INFINITY;
@@ -509,6 +535,8 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     __syncthreads();
     tc5::after_sync();
     if (*given_up && threadIdx.x == 0) {  // the copies under way land before the block ends
+        for (int n = 0; n < H; ++n)
+            if (a.q_by_copy && to[n] > from[n]) ofd::mbar_land(of_half + n * S::kHalfBarriers + 2 * S::kBuffers, 0, 0, ofd::kDefaultWaitLimitNs / 16);
         for (int n = 0; n < S::kStages; ++n) {
             const uint64_t since = ofd::mbar_land(&full[n], 0, 0, ofd::kDefaultWaitLimitNs / 16);
             ofd::mbar_land(&full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
@@ -581,12 +609,12 @@ bool heads_map(CUtensorMap *map, bool bf16, const void *base, int head_dim, int 
 }
 
 template <class T, int DP, int H>
-int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t stream) {
+int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mo, cudaStream_t stream) {
     using S = Shape<DP, H>;
     const auto kernel = attention_kernel<T, DP, H>;
     if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
     const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
-    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mq, mk, mv);
+    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mq, mk, mv, mo);
     if (const int rc = ofe::launched()) return rc;
     if (a.splits == 1) return OPENFISH_B200_OK;
     const long long joins = ((long long)a.max_q * a.q_heads * a.sequences + 3) / 4;
@@ -595,9 +623,9 @@ int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CU
 }
 
 template <class T>
-int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, int halves, cudaStream_t stream) {
-    if (p->head_dim <= 64) return launch<T, 64, 1>(a, mq, mk, mv, stream);
-    return halves == 1 ? launch<T, 128, 1>(a, mq, mk, mv, stream) : launch<T, 128, 2>(a, mq, mk, mv, stream);
+int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mo, int halves, cudaStream_t stream) {
+    if (p->head_dim <= 64) return launch<T, 64, 1>(a, mq, mk, mv, mo, stream);
+    return halves == 1 ? launch<T, 128, 1>(a, mq, mk, mv, mo, stream) : launch<T, 128, 2>(a, mq, mk, mv, mo, stream);
 }
 
 size_t part_bytes(const openfish_b200_attention_t *a, int splits) {
@@ -641,7 +669,7 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
         a.part_lse = a.part + (size_t)a.splits * a.q_rows * a.q_heads * a.head_dim;
     }
     const bool bf16 = p->dtype == OPENFISH_B200_BF16;
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo;
     const int d = p->head_dim, hk = p->kv_heads;
     bool made = p->k_rows == 0  // no keys at all: the kernel copies nothing, but a map has to be one of something
                     ? heads_map(&mk, bf16, p->q, d, 1, 1, 0, 0, 1, kKeys) && heads_map(&mv, bf16, p->q, d, 1, 1, 0, 0, 1, kKeys)
@@ -650,8 +678,11 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     a.q_by_copy = kRows % a.group == 0;
     mq = mk;
     if (a.q_by_copy) made = made && heads_map(&mq, bf16, p->q, d, p->q_heads, p->q_rows, p->q_stride_row, p->q_stride_head, a.group, kRows / a.group);
+    a.out_by_copy = 32 % a.group == 0;
+    mo = mk;
+    if (a.out_by_copy) made = made && heads_map(&mo, bf16, p->out, d, p->q_heads, p->q_rows, p->out_stride_row, p->out_stride_head, a.group, 32 / a.group);
     if (!made) return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
-    return bf16 ? launch_for<__nv_bfloat16>(p, a, mq, mk, mv, halves, (cudaStream_t)stream) : launch_for<__half>(p, a, mq, mk, mv, halves, (cudaStream_t)stream);
+    return bf16 ? launch_for<__nv_bfloat16>(p, a, mq, mk, mv, mo, halves, (cudaStream_t)stream) : launch_for<__half>(p, a, mq, mk, mv, mo, halves, (cudaStream_t)stream);
 }
 
 extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }
