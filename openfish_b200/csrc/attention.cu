@@ -545,13 +545,14 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     if (warp == 4 * H) tc5::tmem_free<1>(tmem, S::kColumns);
 }
 
-// The splits' results joined: out = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A warp to a query and head.
+// The splits' results joined: out = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A block to a query and head, every
+// fourth split to a warp; the sums are formed in the same order every time.
 template <class T>
 __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
-    const int lane = threadIdx.x & 31;
-    const long long per = (long long)a.max_q * a.q_heads;
-    const long long all = per * a.sequences;
-    for (long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); w < all; w += (long long)gridDim.x * 4) {
+    __shared__ float sums[4][128];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long per = (long long)a.max_q * a.q_heads, all = per * a.sequences;
+    for (long long w = blockIdx.x; w < all; w += gridDim.x) {
         const int seq = (int)(w / per), i = (int)(w % per / a.q_heads), head = (int)(w % a.q_heads);
         int q0, nq, k0, nk, lo, hi;
         span(a.q_start, a.q_used, seq, a.q_rows, a.max_q, &q0, &nq);
@@ -559,30 +560,49 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
         span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
         window(a, i, nq, nk, &lo, &hi);
         const long long at = (long long)(q0 + i) * a.q_heads + head, step = (long long)a.q_rows * a.q_heads;
-        float top = -INFINITY;
-        for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_lse[z * step + at]);
+        // a lane to two splits (there are at most 64); -infinity: nothing seen there, or nothing but -infinity
+        float lse[2], top;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) lse[h] = lane + 32 * h < a.splits ? a.part_lse[(lane + 32 * h) * step + at] : -INFINITY;
+        top = fmaxf(lse[0], lse[1]);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         const float from = top == -INFINITY ? 0.f : top;
-        float total = 0.f, acc[4] = {};
-        for (int z = 0; z < a.splits; ++z) {
-            const float lse = a.part_lse[z * step + at];
-            if (lse == -INFINITY) continue;  // nothing seen there (or nothing but -infinity)
-            const float f = ex2(lse - from);
-            total += f;
+        const float f0 = ex2(lse[0] - from), f1 = ex2(lse[1] - from);
+        float total = f0 + f1;
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                if (lane + 32 * n < a.head_dim) acc[n] = fmaf(f, a.part[(z * step + at) * a.head_dim + lane + 32 * n], acc[n]);
+        for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        float acc[4] = {};
+#pragma unroll 4
+        for (int z = warp; z < a.splits; z += 4) {
+            const float f = __shfl_sync(0xffffffffu, z < 32 ? f0 : f1, z & 31);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                if (lane + 32 * n >= a.head_dim) continue;
+                const float o = a.part[(z * step + at) * a.head_dim + lane + 32 * n];
+                acc[n] = f == 0.f ? acc[n] : fmaf(f, o, acc[n]);  // (a split in which nothing was seen has no part)
+            }
         }
-        T *const out = static_cast<T *>(a.out) + (long long)(q0 + i) * a.out_stride_row + head * a.out_stride_head;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-            if (lane + 32 * n < a.head_dim) out[lane + 32 * n] = ofe::from_float<T>(hi > lo ? acc[n] / total : 0.f);
+        for (int n = 0; n < 4; ++n) sums[warp][lane + 32 * n] = acc[n];
+        __syncthreads();
+        const int d = threadIdx.x;
+        if (d < a.head_dim) {
+            const float sum = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+            static_cast<T *>(a.out)[(long long)(q0 + i) * a.out_stride_row + head * a.out_stride_head + d] = ofe::from_float<T>(hi > lo ? sum / total : 0.f);
+        }
+        __syncthreads();
     }
 }
 
 // Halves to a block.
 int halves_for(const openfish_b200_attention_t *a) { return a->head_dim > 64 && (long long)a->max_q * (a->q_heads / a->kv_heads) > kRows ? 2 : 1; }
 
-// Into how many pieces a block's keys go: enough blocks to fill the SMs, four tiles of keys to a piece at least.
+// Into how many pieces a block's keys go: as many as fill the SMs, four tiles of keys to a piece at least.  Where a sequence's
+// queries are one block (single tokens), what they wait for is the keys: two tiles to a piece (one token by 4097 keys, 8
+// heads of 64: 12.7 us, with four tiles 13.9); and where the SMs are nearly full as it is, three times as many blocks of 16 tiles
+// or more even out sequences of different lengths (32 and 64 of 1024 to 8192 keys, 32 / 8 heads of 128: 150 -> 124 and 242 -> 219 us; where all are
+// as long, 339 -> 363).
 int splits_for(const openfish_b200_attention_t *a, int sms) {
     const long long group = a->q_heads / a->kv_heads, halves = halves_for(a), rows = halves * kRows;
     const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64, 1>::kBlocks : Shape<128, 1>::kBlocks / halves);
@@ -593,8 +613,14 @@ int splits_for(const openfish_b200_attention_t *a, int sms) {
         if (seen < keys) keys = seen;
     }
     const long long tiles = (keys + kKeys - 1) / kKeys;
+    const bool one_block = a->max_q * group <= rows;
     long long n = room / blocks;
-    if (n > tiles / 4) n = tiles / 4;
+    if (one_block && n < 4) {
+        long long even = (3 * room + blocks / 2) / blocks;
+        if (even > tiles / 16) even = tiles / 16;
+        if (even > n) n = even;
+    }
+    if (n > tiles / (one_block ? 2 : 4)) n = tiles / (one_block ? 2 : 4);
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
 }
@@ -617,7 +643,7 @@ int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CU
     kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mq, mk, mv, mo);
     if (const int rc = ofe::launched()) return rc;
     if (a.splits == 1) return OPENFISH_B200_OK;
-    const long long joins = ((long long)a.max_q * a.q_heads * a.sequences + 3) / 4;
+    const long long joins = (long long)a.max_q * a.q_heads * a.sequences;
     attention_join_kernel<T><<<(unsigned)(joins < 16384 ? joins : 16384), 128, 0, stream>>>(a);
     return ofe::launched();
 }
