@@ -600,9 +600,9 @@ int halves_for(const openfish_b200_attention_t *a) { return a->head_dim > 64 && 
 
 // Into how many pieces a block's keys go: as many as fill the SMs, four tiles of keys to a piece at least.  Where a sequence's
 // queries are one block (single tokens), what they wait for is the keys: two tiles to a piece (one token by 4097 keys, 8
-// heads of 64: 12.7 us, with four tiles 13.9); and where the SMs are nearly full as it is, three times as many blocks of 16 tiles
-// or more even out sequences of different lengths (32 and 64 of 1024 to 8192 keys, 32 / 8 heads of 128: 150 -> 124 and 242 -> 219 us; where all are
-// as long, 339 -> 363).
+// heads of 64: 12.7 us, with four tiles 13.9); and where the SMs are nearly full as it is, three pieces of 16 tiles or more even
+// out sequences of different lengths (one token each by 1024 to 8192 keys, 32 / 8 heads of 128, us by one, two, three, four pieces: 64
+// sequences 246, 217, 214, 214, 32 sequences 195, 162, 143, 162; 64 of 8192 keys all 347, 355, 370, 373).
 int splits_for(const openfish_b200_attention_t *a, int sms) {
     const long long group = a->q_heads / a->kv_heads, halves = halves_for(a), rows = halves * kRows;
     const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64, 1>::kBlocks : Shape<128, 1>::kBlocks / halves);
@@ -616,8 +616,7 @@ int splits_for(const openfish_b200_attention_t *a, int sms) {
     const bool one_block = a->max_q * group <= rows;
     long long n = room / blocks;
     if (one_block && n < 4) {
-        long long even = (3 * room + blocks / 2) / blocks;
-        if (even > tiles / 16) even = tiles / 16;
+        const long long even = tiles / 16 < 3 ? tiles / 16 : 3;
         if (even > n) n = even;
     }
     if (n > tiles / (one_block ? 2 : 4)) n = tiles / (one_block ? 2 : 4);

@@ -46,7 +46,7 @@ static int bad_attention_sizes(const char *func, const openfish_b200_attention_t
         return refuse(func, OPENFISH_B200_ERR_SHAPE, "q_heads must be a multiple of kv_heads, both at least 1");
     if (a->sequences < 0 || a->max_q < 0 || a->max_k < 0 || a->q_rows < 0 || a->k_rows < 0)
         return refuse(func, OPENFISH_B200_ERR_SHAPE, "negative extent");
-    if (a->q_rows > INT_MAX || a->k_rows > INT_MAX || a->max_k > INT_MAX / 4 || (double)a->max_q * a->q_heads > 1e9 ||
+    if (a->q_rows > INT_MAX - 65536 || a->k_rows > INT_MAX - 65536 || a->max_k > INT_MAX / 4 || (double)a->max_q * a->q_heads > 1e9 ||
         ((double)a->max_q * a->q_heads / a->kv_heads / 128 + 1) * a->kv_heads * a->sequences > 1e9)
         return refuse(func, OPENFISH_B200_ERR_TOO_LONG, "more rows than the kernels count (2^31 rows, 2^29 keys and 10^9 query heads of one sequence, 10^9 tiles of 128)");
     if (!(a->scale > 0.f) || isinf(a->scale)) return refuse(func, OPENFISH_B200_ERR_ARGUMENT, "scale must be finite and above zero");
