@@ -34,7 +34,7 @@ __device__ int g_status;  // of the kernels on this device: a wait that ran out
 
 constexpr int kRows = 128;  // of a half
 constexpr int kKeys = 64;   // of a tile
-constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled: weights up to 256
+constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled
 
 struct Args {
     const int32_t *q_start, *k_start, *q_used, *k_used;
@@ -76,10 +76,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// Two weights 2^(c s - c m) as the matrix unit takes them, added to their row's sum (before they are rounded).
+// Two weights 2^(c s - c m) as the matrix unit takes them, added to their row's sum before they are rounded.
 template <class T>
 __device__ __forceinline__ uint32_t weights(float u, float w, float c, float shift, float2 &sum) {
-    float2 z = fma2({u, w}, {c, c}, {shift, shift});
+    float2 z = {fmaf(u, c, shift), fmaf(w, c, shift)};
     z.x = ex2(z.x);
     z.y = ex2(z.y);
     sum = add2(sum, z);
@@ -356,29 +356,26 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             if (warp_there) {  // (else nothing but rows that are not there: their weights are whatever lies in the place)
                 const uint32_t s_at = tmem + lanes + buffer * kKeys;
                 const int j0 = base + t * kKeys;
-                // In a tile that every row sees all of, the weights are worked out with the maximum there was before, and
-                // the tile's own maximum beside them.  It hardly ever outgrows the other by as much as it may.
+                // In a tile that every row sees all of, the weights are worked out with the maximum there was before.  It is good
+                // enough while their sum is below 2^15: then so is each of them, which every type can hold.
                 bool careful = u == 0 || last_lo > j0 || first_hi < j0 + kKeys;
                 if (!careful) {
                     uint32_t s[2][32], p[2][16];
                     tc5::ld64(s[0], s[1], s_at);
                     const float shift = -m * a.c;
-                    float top[2] = {-INFINITY, -INFINITY};
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float u = __uint_as_float(s[n][e * 2]), w = __uint_as_float(s[n][e * 2 + 1]);
-                            top[e & 1] = max3(top[e & 1], u, w);
-                            p[n][e] = weights<T>(u, w, a.c, shift, sum[e & 1]);
-                        }
-                    careful = __any_sync(0xffffffffu, !((fmaxf(top[0], top[1]) - m) * a.c <= kLazy));
+                        for (int e = 0; e < 16; ++e)
+                            p[n][e] = weights<T>(__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1]), a.c, shift, sum[e & 1]);
+                    sum[0] = add2(sum[0], sum[1]);
+                    const float tile_sum = sum[0].x + sum[0].y;
+                    careful = __any_sync(0xffffffffu, !(tile_sum <= 32768.f));  // (nor if it is no number)
                     if (!careful) {
                         tc5::st16(s_at, p[0]);
                         tc5::st16(s_at + 16, p[1]);
-                        sum[0] = add2(sum[0], sum[1]);
-                        l += sum[0].x + sum[0].y;
+                        l += tile_sum;
                     }
                 }
                 if (careful) {
@@ -613,7 +610,7 @@ int splits_for(const openfish_b200_attention_t *a, int sms) {
         if (seen < keys) keys = seen;
     }
     const long long tiles = (keys + kKeys - 1) / kKeys;
-    const bool one_block = a->max_q * group <= rows;
+    const bool one_block = a->max_q * group <= kRows;
     long long n = room / blocks;
     if (one_block && n < 4) {
         const long long even = tiles / 16 < 3 ? tiles / 16 : 3;
