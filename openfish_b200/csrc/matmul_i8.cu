@@ -7,6 +7,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "encoder_device.cuh"
 #include "tc5.cuh"
 
@@ -240,13 +242,39 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                         tc5::store_commit();
                     }
                 } else {
-                    // rows of out that start anywhere: two results to a lane, a row to an instruction
+                    // Rows of out that start anywhere: a row to an instruction, two results to a lane; a row that starts off a 4-byte
+                    // boundary takes two instructions.  (53312 x 1538 and 1537 x 512: 68 and 74 us, 1536 by tiled copies 46.)
                     __syncwarp();
-                    T *const out = static_cast<T *>(a.out) + (long long)m0 * a.out_stride + n0 + c;
-                    for (int r = 0; r < 32 && m0 + r < a.rows; ++r) {
-                        const T *const from = reinterpret_cast<const T *>(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4)) + (lane & 3) * 2;
-                        if (n0 + c + 2 * lane < a.cols) out[r * a.out_stride + 2 * lane] = from[0];
-                        if (n0 + c + 2 * lane + 1 < a.cols) out[r * a.out_stride + 2 * lane + 1] = from[1];
+                    const int n = n0 + c, high = min(32, a.rows - m0), wide = min(64, a.cols - n);
+                    uint16_t *out = static_cast<uint16_t *>(a.out) + (long long)m0 * a.out_stride + n;
+                    if (high == 32 && wide == 64) {
+                        // (n and the tile's first row are even: which rows start in front of a boundary is the same in every tile)
+                        const auto rows = [&](auto first_odd, auto alternate) {
+#pragma unroll 1
+                            for (int r0 = 0; r0 < 32; r0 += 8) {
+                                uint32_t two[8];
+#pragma unroll
+                                for (int r = 0; r < 8; ++r) two[r] = *reinterpret_cast<const uint32_t *>(to + (r0 + r) * 128 + (((lane >> 2) ^ r) << 4) + (lane & 3) * 4);
+#pragma unroll
+                                for (int r = 0; r < 8; ++r, out += a.out_stride) {
+                                    if (first_odd.value != (alternate.value && (r & 1))) {
+                                        out[2 * lane] = (uint16_t)two[r];
+                                        out[2 * lane + 1] = (uint16_t)(two[r] >> 16);
+                                    } else {
+                                        *reinterpret_cast<uint32_t *>(out + 2 * lane) = two[r];
+                                    }
+                                }
+                            }
+                        };
+                        const bool odd = (uintptr_t)a.out & 2, alternate = a.out_stride & 1;
+                        if (alternate) odd ? rows(std::true_type(), std::true_type()) : rows(std::false_type(), std::true_type());
+                        else odd ? rows(std::true_type(), std::false_type()) : rows(std::false_type(), std::false_type());
+                    } else {
+                        for (int r = 0; r < high; ++r, out += a.out_stride) {
+                            const uint32_t two = *reinterpret_cast<const uint32_t *>(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                            if (2 * lane < wide) out[2 * lane] = (uint16_t)two;
+                            if (2 * lane + 1 < wide) out[2 * lane + 1] = (uint16_t)(two >> 16);
+                        }
                     }
                     __syncwarp();
                 }
