@@ -40,7 +40,8 @@ struct Args {
     const int32_t *q_start, *k_start, *q_used, *k_used;
     const void *q, *k, *v;
     void *out;
-    float *part, *part_lse;  // of a split: [split][q_rows][q_heads][head_dim] and [split][q_rows][q_heads]
+    float *part, *part_lse;  // of a split: [split][sequences * max_q][q_heads][head_dim] and [split][sequences * max_q][q_heads]
+    long long part_step;     // sequences * max_q * q_heads
     long long q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head, out_stride_row, out_stride_head;
     int q_rows, k_rows, q_heads, kv_heads, group, head_dim, sequences, max_q, max_k, left, right;
     ofe::Divider by_group;
@@ -456,9 +457,9 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             const int in_lo = max(my_lo, base), in_hi = min(my_hi, base + count * kKeys);  // of this split
             const bool sees = there && in_hi > in_lo;
             const float back = sees ? 1.f / l : 0.f;
-            const long long at = (long long)(q0 + i) * a.q_heads + head;  // of [q_rows][q_heads]
+            const long long at = split * a.part_step + ((long long)seq * a.max_q + i) * a.q_heads + head;
             T *const out = static_cast<T *>(a.out) + (long long)(q0 + i) * a.out_stride_row + head * a.out_stride_head;
-            float *const part = a.part + ((long long)split * a.q_rows * a.q_heads + at) * a.head_dim;
+            float *const part = a.part + at * a.head_dim;
             bool bad = false;
             // A warp whose rows are all there puts them where its queries were, and a tiled copy takes them out; else each thread
             // writes its own.
@@ -515,16 +516,16 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                 const int who = __ffs(again) - 1;
                 const int rr = half0 + (warp & 3) * 32 + who, ii = a.by_group.quotient(rr), hh = kh * a.group + rr - ii * a.group;
                 const int klo = __shfl_sync(0xffffffffu, in_lo, who), khi = __shfl_sync(0xffffffffu, in_hi, who);
-                const long long aa = (long long)(q0 + ii) * a.q_heads + hh;
+                const long long aa = split * a.part_step + ((long long)seq * a.max_q + ii) * a.q_heads + hh;
                 const float2 ml = redo_row<T>(static_cast<const T *>(a.q) + (long long)(q0 + ii) * a.q_stride_row + hh * a.q_stride_head,
                                               static_cast<const T *>(a.k) + (long long)k0 * a.k_stride_row + kh * a.k_stride_head,
                                               static_cast<const T *>(a.v) + (long long)k0 * a.v_stride_row + kh * a.v_stride_head, a.k_stride_row,
                                               a.v_stride_row, a.head_dim, a.c, klo, khi,
-                                              a.part + ((long long)split * a.q_rows * a.q_heads + aa) * a.head_dim,
+                                              a.part + aa * a.head_dim,
                                               a.splits > 1 ? nullptr : static_cast<T *>(a.out) + (long long)(q0 + ii) * a.out_stride_row + hh * a.out_stride_head);
                 if (lane == who) lse = ml.x * a.c + log2f(ml.y);
             }
-            if (a.splits > 1 && there) a.part_lse[(long long)split * a.q_rows * a.q_heads + at] = lse;
+            if (a.splits > 1 && there) a.part_lse[at] = lse;
         }
     }
     __syncwarp();
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
         if (i >= nq) continue;
         span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
         window(a, i, nq, nk, &lo, &hi);
-        const long long at = (long long)(q0 + i) * a.q_heads + head, step = (long long)a.q_rows * a.q_heads;
+        const long long at = w, step = a.part_step;
         // a lane to two splits (there are at most 64); -infinity: nothing seen there, or nothing but -infinity
         float lse[2], top;
 #pragma unroll
@@ -651,7 +652,7 @@ int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensor
 }
 
 size_t part_bytes(const openfish_b200_attention_t *a, int splits) {
-    return splits == 1 ? 0 : (size_t)splits * a->q_rows * a->q_heads * (a->head_dim + 1) * sizeof(float);
+    return splits == 1 ? 0 : (size_t)splits * a->sequences * a->max_q * a->q_heads * (a->head_dim + 1) * sizeof(float);
 }
 
 }  // namespace
@@ -683,12 +684,13 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     const int halves = halves_for(p);
     a.tiles = (int)(((long long)p->max_q * a.group + halves * kRows - 1) / (halves * kRows));
     a.splits = splits_for(p, sms);
+    a.part_step = (long long)p->sequences * p->max_q * p->q_heads;
     a.part_lse = static_cast<float *>(p->workspace);
     a.part = a.part_lse;
     if (a.splits > 1) {
         // sums first: their rows are read and written 16 bytes at a time
         a.part = static_cast<float *>(p->workspace);
-        a.part_lse = a.part + (size_t)a.splits * a.q_rows * a.q_heads * a.head_dim;
+        a.part_lse = a.part + a.splits * a.part_step * a.head_dim;
     }
     const bool bf16 = p->dtype == OPENFISH_B200_BF16;
     CUtensorMap mq, mk, mv, mo;

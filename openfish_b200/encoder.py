@@ -3,7 +3,8 @@ sequences, the product of 8-bit integers, and the residual norm that feeds it.
 
 Tensors are torch CUDA tensors of one device; the calls queue their kernels on ``stream`` (a torch.cuda.Stream of that
 device; its current stream by default) and return.  Arguments that cannot be served raise before anything is queued:
-TypeError and ValueError for what is no such tensor, OpenfishError for what the library refuses.
+TypeError and ValueError for what is no such tensor, OpenfishError for what the library refuses.  The operators serve: no
+gradient passes through them.
 """
 import contextlib
 import ctypes as C

@@ -293,6 +293,19 @@ def test_the_workspace_is_asked_for_and_checked(native_lib):
     assert (room[need:] == 255).all()
 
 
+def test_the_workspace_goes_by_the_queries_that_there_can_be(native_lib):
+    # one sequence of at most two queries in a tensor of many rows
+    q, k, v = make(100000, 8, 64, torch.float16, 1), make(30000, 2, 64, torch.float16, 2), make(30000, 2, 64, torch.float16, 3)
+    at = torch.tensor([77777, 77779], dtype=torch.int32, device="cuda")
+    keys = starts([30000])[1]
+    assert native_lib.attention_workspace_bytes(q, k, v, at, keys, 2, 30000, causal=True) <= 64 * 2 * 8 * 65 * 4
+    out = torch.full_like(q, 7.0)
+    native_lib.attention(q, k, v, at, keys, 2, 30000, causal=True, out=out)
+    ref = attention_reference(q[77777:77779], k, v, [0, 2], [0, 30000], window=(-1, 0))
+    assert close(out[77777:77779], ref[0], attention_bound(ref, torch.float16, 30000))
+    assert (out[:77777] == 7).all() and (out[77779:] == 7).all()
+
+
 def test_a_cache_beyond_32_bits_of_elements(native_lib):
     # the keys of the second sequence lie 2^32 elements in
     rows = 2 ** 32 // 128 + 4000
