@@ -211,8 +211,8 @@ enum openfish_b200_dtype { OPENFISH_B200_F16 = 0, OPENFISH_B200_BF16 = 1 };
  * their values (infinities and NaN included).
  *
  * q [q_rows][q_heads][head_dim], k and v [k_rows][kv_heads][head_dim], out like q, all of type `dtype`, the head_dim
- * elements of a head next to each other, 16-byte aligned, strides multiples of 8 and positive.  head_dim: a multiple
- * of 8 up to 128.  Sequence s has the queries q_start[s] .. q_start[s] + n - 1, n = q_used[s], or
+ * elements of a head next to each other, 16-byte aligned, strides multiples of 8 and positive (out's such that no
+ * two rows or heads share an element).  head_dim: a multiple of 8 up to 128.  Sequence s has the queries q_start[s] .. q_start[s] + n - 1, n = q_used[s], or
  * q_start[s + 1] - q_start[s] where q_used is NULL, and its keys likewise: q_used and k_used are for padded batches and
  * caches with room left; they are cut to the room that the starts give.  Starts and used lengths are in device memory and are read by the kernels; starts have sequences + 1
  * entries, do not fall, and lie in 0 .. rows.  Rows of out behind a sequence's last query are left as they were.

@@ -19,8 +19,8 @@ static int bad_dtype(const char *func, int dtype) {
 
 /* A tensor [rows][heads][head_dim]: a stride counts only where there is a second element along it.  The limit on a
  * stride is that of a tensor map (40 bits of bytes). */
-static int bad_heads(const char *func, const char *name, const void *p, long long rows, int heads, int head_dim,
-                     long long stride_row, long long stride_head) {
+static int bad_heads(const char *func, const char *name, const void *p, long long rows, int heads, long long stride_row,
+                     long long stride_head) {
     char msg[160];
     if (!p) {
         snprintf(msg, sizeof(msg), "%s must not be NULL", name);
@@ -32,8 +32,14 @@ static int bad_heads(const char *func, const char *name, const void *p, long lon
         snprintf(msg, sizeof(msg), "%s must be 16-byte aligned, its strides positive multiples of 8", name);
         return refuse(func, OPENFISH_B200_ERR_LAYOUT, msg);
     }
-    (void)head_dim;
     return 0;
+}
+/* Of a tensor that is written, the rows and heads lie next to or inside one another's gaps: no element has two places. */
+static int elements_meet(long long rows, int heads, int head_dim, long long stride_row, long long stride_head) {
+    if (rows < 2) return heads > 1 && stride_head < head_dim;
+    if (heads < 2) return stride_row < head_dim;
+    if (stride_head <= stride_row) return stride_head < head_dim || stride_row < (heads - 1) * stride_head + head_dim;
+    return stride_row < head_dim || (stride_head - head_dim) / stride_row < rows - 1;
 }
 
 /* What does not need the pointers. */
@@ -73,12 +79,16 @@ void openfish_b200_attention(void *cuda_stream, const openfish_b200_attention_t 
         refuse(__func__, OPENFISH_B200_ERR_LAYOUT, "starts and used lengths must be aligned to their type");
         return;
     }
-    if (bad_heads(__func__, "q", a->q, a->q_rows, a->q_heads, a->head_dim, a->q_stride_row, a->q_stride_head) ||
-        bad_heads(__func__, "out", a->out, a->q_rows, a->q_heads, a->head_dim, a->out_stride_row, a->out_stride_head))
+    if (bad_heads(__func__, "q", a->q, a->q_rows, a->q_heads, a->q_stride_row, a->q_stride_head) ||
+        bad_heads(__func__, "out", a->out, a->q_rows, a->q_heads, a->out_stride_row, a->out_stride_head))
         return;
+    if (elements_meet(a->q_rows, a->q_heads, a->head_dim, a->out_stride_row, a->out_stride_head)) {
+        refuse(__func__, OPENFISH_B200_ERR_LAYOUT, "rows and heads of out must not overlap");
+        return;
+    }
     if (a->k_rows > 0 &&
-        (bad_heads(__func__, "k", a->k, a->k_rows, a->kv_heads, a->head_dim, a->k_stride_row, a->k_stride_head) ||
-         bad_heads(__func__, "v", a->v, a->k_rows, a->kv_heads, a->head_dim, a->v_stride_row, a->v_stride_head)))
+        (bad_heads(__func__, "k", a->k, a->k_rows, a->kv_heads, a->k_stride_row, a->k_stride_head) ||
+         bad_heads(__func__, "v", a->v, a->k_rows, a->kv_heads, a->v_stride_row, a->v_stride_head)))
         return;
     const size_t need = ofb_attention_workspace(a);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16))) {

@@ -46,7 +46,13 @@ def _packer(args):
     code = {C.c_int: "i", C.c_float: "f", C.c_longlong: "q", C.c_void_p: "P", C.c_size_t: "N"}
     packer = struct.Struct("@" + "".join(code[t] for _, t in args._fields_))
     assert packer.size == C.sizeof(args)
-    return packer.pack
+
+    def pack(*fields):
+        try:
+            return packer.pack(*fields)
+        except (struct.error, OverflowError) as e:
+            raise ValueError("a size or number that the library does not take: %s" % e) from None
+    return pack
 
 
 _pack_attention, _pack_matmul_i8, _pack_norm = _packer(AttentionArgs), _packer(MatmulI8Args), _packer(NormArgs)

@@ -127,3 +127,23 @@ def test_host_tensors_are_refused(native_lib):
         native_lib.matmul_i8(q, torch.ones(4), q, torch.ones(4))
     with pytest.raises(TypeError):
         native_lib.attention(x[:, None], x[:, None], x[:, None], starts, starts, 4, 4)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(out_stride_row=448), LAYOUT), (dict(out_stride_head=56), LAYOUT), (dict(out_stride_row=64, out_stride_head=64), LAYOUT), (dict(q_heads=4, out_stride_row=248), LAYOUT),
+    (dict(out_stride_row=64, out_stride_head=64 * 19), LAYOUT), (dict(out_stride_row=56, out_stride_head=56 * 20), LAYOUT), (dict(kv_heads=1, q_heads=1, out_stride_row=56), LAYOUT),
+    (dict(q_rows=1, out_stride_head=56), LAYOUT)])
+def test_attention_refuses_results_that_share_places(native_lib, lib, change, status):
+    lib.openfish_b200_attention(None, C.byref(attention(native_lib, **change)))
+    assert lib.openfish_b200_last_status() == status, lib.openfish_b200_error_text()
+    assert b"overlap" in lib.openfish_b200_error_text()
+
+
+@pytest.mark.parametrize("pack,args", [("_pack_attention", "AttentionArgs"), ("_pack_matmul_i8", "MatmulI8Args"), ("_pack_norm", "NormArgs")])
+@pytest.mark.parametrize("number", [1 << 31, 1 << 70, 2.5, None])
+def test_numbers_that_no_field_holds_are_refused(native_lib, pack, args, number):
+    fields = [0] * len(getattr(native_lib.encoder, args)._fields_)
+    assert len(getattr(native_lib.encoder, pack)(*fields)) == C.sizeof(getattr(native_lib.encoder, args))
+    fields[1] = number
+    with pytest.raises(ValueError):
+        getattr(native_lib.encoder, pack)(*fields)
