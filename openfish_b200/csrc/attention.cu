@@ -548,6 +548,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
 template <class T>
 __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
     __shared__ float sums[4][128];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits are done, and what they wrote is there
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long per = (long long)a.max_q * a.q_heads, all = per * a.sequences;
     for (long long w = blockIdx.x; w < all; w += gridDim.x) {
@@ -600,7 +601,8 @@ int halves_for(const openfish_b200_attention_t *a) { return a->head_dim > 64 && 
 // queries are one block (single tokens), what they wait for is the keys: two tiles to a piece (one token by 4097 keys, 8
 // heads of 64: 12.7 us, with four tiles 13.9); and where the SMs are nearly full as it is, three pieces of 16 tiles or more even
 // out sequences of different lengths (one token each by 1024 to 8192 keys, 32 / 8 heads of 128, us by one, two, three, four pieces: 64
-// sequences 246, 217, 214, 214, 32 sequences 195, 162, 143, 162; 64 of 8192 keys all 347, 355, 370, 373).
+// sequences 246, 217, 214, 214, 32 sequences 195, 162, 143, 162; 64 of 8192 keys all 347, 355, 370, 373).  Four rounds over the SMs even
+// themselves out (by one and three: 128 sequences 450, 450, 256 of 512 to 4096 keys 434, 480).
 int splits_for(const openfish_b200_attention_t *a, int sms) {
     const long long group = a->q_heads / a->kv_heads, halves = halves_for(a), rows = halves * kRows;
     const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64, 1>::kBlocks : Shape<128, 1>::kBlocks / halves);
@@ -613,7 +615,7 @@ int splits_for(const openfish_b200_attention_t *a, int sms) {
     const long long tiles = (keys + kKeys - 1) / kKeys;
     const bool one_block = a->max_q * group <= kRows;
     long long n = room / blocks;
-    if (one_block && n < 4) {
+    if (one_block && n < 4 && blocks < 4 * room) {
         const long long even = tiles / 16 < 3 ? tiles / 16 : 3;
         if (even > n) n = even;
     }
@@ -641,8 +643,17 @@ int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CU
     if (const int rc = ofe::launched()) return rc;
     if (a.splits == 1) return OPENFISH_B200_OK;
     const long long joins = (long long)a.max_q * a.q_heads * a.sequences;
-    attention_join_kernel<T><<<(unsigned)(joins < 16384 ? joins : 16384), 128, 0, stream>>>(a);
-    return ofe::launched();
+    // its blocks come to the SMs while the last ones before them leave (one token by 4097 keys: 14.8 us, without 15.4)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(joins < 16384 ? joins : 16384));
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return ofe::cuda_status(cudaLaunchKernelEx(&cfg, attention_join_kernel<T>, a));
 }
 
 template <class T>
