@@ -18,6 +18,8 @@
 // two share a block and its tiles, for the copies' way into shared memory and the products' way out of it are what bounds
 // these heads: 48 cycles for each 128 x 64 x 16 of Q K^T (6 KB), 64 for 128 x 128 x 16 of P V.  Where there are rows for one half only (single
 // tokens), a block has one, and an SM two blocks.
+//
+// Single tokens with one or two heads to a key head have no use for tiles of 128 rows: attention_few_kernel.
 #include <math.h>
 #include <stdint.h>
 
@@ -543,6 +545,155 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     if (warp == 4 * H) tc5::tmem_free<1>(tmem, S::kColumns);
 }
 
+// A single token to a sequence, R heads to a key head, which all see the same keys: what counts is to read those once.  LK lanes
+// have 16 bytes each of a key and of its value, a slot of that many lanes takes every (kSlots)th key and keeps a maximum, a sum and
+// results of its own, in fp32; the slots are joined at the end.  kAhead keys and values are on the way to every lane.
+template <int LK, int R>
+struct FewShape {
+    static constexpr int kWarps = 4, kThreads = 32 * kWarps, kInWarp = 32 / LK, kSlots = kWarps * kInWarp, kAhead = 4;
+    static constexpr int kBlocks = R == 1 ? 7 : 5;  // to an SM, by their registers
+};
+
+template <class T, int LK, int R>
+__global__ void __launch_bounds__(FewShape<LK, R>::kThreads, FewShape<LK, R>::kBlocks) attention_few_kernel(const Args a) {
+    using S = FewShape<LK, R>;
+    __shared__ float sums[S::kWarps][R][LK * 8], tops[S::kWarps][R], totals[S::kWarps][R];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp * S::kInWarp + lane / LK, at = lane % LK * 8;
+    const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits, kh = pair % a.kv_heads, seq = pair / a.kv_heads;
+    int q0, nq, k0, nk, lo, hi;
+    span(a.q_start, a.q_used, seq, a.q_rows, a.max_q, &q0, &nq);
+    if (nq == 0) return;
+    span(a.k_start, a.k_used, seq, a.k_rows, a.max_k, &k0, &nk);
+    window(a, 0, nq, nk, &lo, &hi);
+    const int tiles = (max(hi - lo, 0) + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
+    const int first = lo + min(split * per, tiles) * kKeys, last = min(first + per * kKeys, hi);
+    const bool mine = at < a.head_dim;
+
+    float2 q[R][4], acc[R][4] = {};
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (mine)
+            w = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)q0 * a.q_stride_row + (kh * R + r) * a.q_stride_head + at);
+        q[r][0] = ofe::unpack<T>(w.x);
+        q[r][1] = ofe::unpack<T>(w.y);
+        q[r][2] = ofe::unpack<T>(w.z);
+        q[r][3] = ofe::unpack<T>(w.w);
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+    }
+    const T *const keys = static_cast<const T *>(a.k) + (long long)k0 * a.k_stride_row + kh * a.k_stride_head + at;
+    const T *const values = static_cast<const T *>(a.v) + (long long)k0 * a.v_stride_row + kh * a.v_stride_head + at;
+    for (int j0 = first; j0 < last; j0 += S::kSlots * S::kAhead) {
+        uint4 kw[S::kAhead], vw[S::kAhead];
+        float z[R][S::kAhead];
+#pragma unroll
+        for (int n = 0; n < S::kAhead; ++n) {
+            const int j = j0 + n * S::kSlots + slot;
+            kw[n] = vw[n] = make_uint4(0, 0, 0, 0);
+            if (j < last && mine) {
+                kw[n] = __ldcs(reinterpret_cast<const uint4 *>(keys + j * a.k_stride_row));
+                vw[n] = __ldcs(reinterpret_cast<const uint4 *>(values + j * a.v_stride_row));
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < S::kAhead; ++n) {
+            const float2 f[4] = {ofe::unpack<T>(kw[n].x), ofe::unpack<T>(kw[n].y), ofe::unpack<T>(kw[n].z), ofe::unpack<T>(kw[n].w)};
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float2 dot = {0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dot = fma2(q[r][e], f[e], dot);
+                z[r][n] = dot.x + dot.y;
+            }
+        }
+#pragma unroll
+        for (int d = LK / 2; d > 0; d >>= 1)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int n = 0; n < S::kAhead; ++n) z[r][n] += __shfl_xor_sync(0xffffffffu, z[r][n], d);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float top = m[r];
+#pragma unroll
+            for (int n = 0; n < S::kAhead; ++n) {
+                if (j0 + n * S::kSlots + slot >= last) z[r][n] = -INFINITY;
+                top = fmaxf(top, z[r][n]);
+            }
+            const float fade = m[r] == top ? 1.f : ex2((m[r] - top) * a.c), from = top == -INFINITY ? 0.f : top;
+            m[r] = top;
+            l[r] *= fade;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[r][e] = ofe::mul2(acc[r][e], {fade, fade});
+#pragma unroll
+            for (int n = 0; n < S::kAhead; ++n) {
+                z[r][n] = ex2((z[r][n] - from) * a.c);
+                l[r] += z[r][n];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < S::kAhead; ++n) {
+            const float2 f[4] = {ofe::unpack<T>(vw[n].x), ofe::unpack<T>(vw[n].y), ofe::unpack<T>(vw[n].z), ofe::unpack<T>(vw[n].w)};
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[r][e] = fma2({z[r][n], z[r][n]}, f[e], acc[r][e]);
+        }
+    }
+    // ---- the slots of a warp, then the warps
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int d = LK; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float fade = m[r] == top ? 1.f : ex2((m[r] - top) * a.c);
+        l[r] *= fade;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[r][e] = ofe::mul2(acc[r][e], {fade, fade});
+#pragma unroll
+        for (int d = LK; d < 32; d <<= 1) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[r][e].x += __shfl_xor_sync(0xffffffffu, acc[r][e].x, d);
+                acc[r][e].y += __shfl_xor_sync(0xffffffffu, acc[r][e].y, d);
+            }
+        }
+        if (lane < LK) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<float2 *>(&sums[warp][r][at + e * 2]) = acc[r][e];
+            if (lane == 0) {
+                tops[warp][r] = top;
+                totals[warp][r] = l[r];
+            }
+        }
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < R * a.head_dim; n += S::kThreads) {
+        const int r = n / a.head_dim, d = n - r * a.head_dim, head = kh * R + r;
+        float top = -INFINITY, total = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, tops[w][r]);
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w) {
+            const float f = tops[w][r] == top ? 1.f : ex2((tops[w][r] - top) * a.c);
+            total = fmaf(totals[w][r], f, total);
+            sum = fmaf(sums[w][r][d], f, sum);
+        }
+        // (a sum that is no number makes every element none)
+        const float o = last <= first ? 0.f : total == total ? sum / total : NAN;
+        if (a.splits == 1) {
+            static_cast<T *>(a.out)[(long long)q0 * a.out_stride_row + head * a.out_stride_head + d] = ofe::from_float<T>(o);
+        } else {
+            const long long to = split * a.part_step + (long long)seq * a.max_q * a.q_heads + head;
+            a.part[to * a.head_dim + d] = o;
+            if (d == 0) a.part_lse[to] = last <= first ? -INFINITY : top * a.c + log2f(total);
+        }
+    }
+}
+
 // The splits' results joined: out = sum_z 2^(lse_z - max) o_z / sum_z 2^(lse_z - max).  A block to a query and head, every
 // fourth split to a warp; the sums are formed in the same order every time.
 template <class T>
@@ -594,18 +745,28 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const Args a) {
     }
 }
 
+// Whether the calls' rows are few enough for attention_few_kernel: a token to a sequence, as many heads to a key head as its lanes have
+// the instructions for.  By it and by the tiles, us: heads of 64, one, two, four to a key head, 256 sequences of 256 to 2048 keys 102 / 153,
+// 119 / 183, 175 / 163, one of 4097 keys 8.4 / 12.7, 10.6 / 17.7, 11.1 / 13.1; heads of 128, one, two, four, 64 sequences of 1024 to 8192 keys
+// 720 (6.6 TB/s) / 841, 243 / 206, 346 / 211.
+bool few_for(const openfish_b200_attention_t *a) {
+    const int group = a->q_heads / a->kv_heads;
+    return a->max_q == 1 && (group == 1 || (group == 2 && a->head_dim <= 64));
+}
+
 // Halves to a block.
 int halves_for(const openfish_b200_attention_t *a) { return a->head_dim > 64 && (long long)a->max_q * (a->q_heads / a->kv_heads) > kRows ? 2 : 1; }
 
 // Into how many pieces a block's keys go: as many as fill the SMs, four tiles of keys to a piece at least.  Where a sequence's
 // queries are one block (single tokens), what they wait for is the keys: two tiles to a piece (one token by 4097 keys, 8
-// heads of 64: 12.7 us, with four tiles 13.9); and where the SMs are nearly full as it is, three pieces of 16 tiles or more even
+// heads of 64 by the matrix instructions: 12.7 us, with four tiles 13.9); and where the SMs are nearly full as it is, three pieces of 16 tiles or more even
 // out sequences of different lengths (one token each by 1024 to 8192 keys, 32 / 8 heads of 128, us by one, two, three, four pieces: 64
 // sequences 246, 217, 214, 214, 32 sequences 195, 162, 143, 162; 64 of 8192 keys all 347, 355, 370, 373).  Four rounds over the SMs even
 // themselves out (by one and three: 128 sequences 450, 450, 256 of 512 to 4096 keys 434, 480).
 int splits_for(const openfish_b200_attention_t *a, int sms) {
     const long long group = a->q_heads / a->kv_heads, halves = halves_for(a), rows = halves * kRows;
-    const long long room = (long long)sms * (a->head_dim <= 64 ? Shape<64, 1>::kBlocks : Shape<128, 1>::kBlocks / halves);
+    const long long room = (long long)sms * (few_for(a) ? (group == 1 ? FewShape<8, 1>::kBlocks : FewShape<8, 2>::kBlocks)
+                                             : a->head_dim <= 64 ? Shape<64, 1>::kBlocks : Shape<128, 1>::kBlocks / halves);
     const long long blocks = (a->max_q * group + rows - 1) / rows * a->kv_heads * a->sequences;
     long long keys = a->max_k;
     if (a->window_left >= 0 && a->window_right >= 0) {
@@ -633,17 +794,11 @@ bool heads_map(CUtensorMap *map, bool bf16, const void *base, int head_dim, int 
     return tc5::make_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box);
 }
 
-template <class T, int DP, int H>
-int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mo, cudaStream_t stream) {
-    using S = Shape<DP, H>;
-    const auto kernel = attention_kernel<T, DP, H>;
-    if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
-    const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
-    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mq, mk, mv, mo);
-    if (const int rc = ofe::launched()) return rc;
+template <class T>
+int join(const Args &a, cudaStream_t stream) {
     if (a.splits == 1) return OPENFISH_B200_OK;
     const long long joins = (long long)a.max_q * a.q_heads * a.sequences;
-    // its blocks come to the SMs while the last ones before them leave (one token by 4097 keys: 14.8 us, without 15.4)
+    // its blocks come to the SMs while the last ones before them leave (one token by 4097 keys by the tiles: 14.8 us, without 15.4)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(joins < 16384 ? joins : 16384));
     cfg.blockDim = dim3(128);
@@ -656,10 +811,34 @@ int launch(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CU
     return ofe::cuda_status(cudaLaunchKernelEx(&cfg, attention_join_kernel<T>, a));
 }
 
+template <class T, int DP, int H>
+int launch_tiles(const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mo, cudaStream_t stream) {
+    using S = Shape<DP, H>;
+    const auto kernel = attention_kernel<T, DP, H>;
+    if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
+    const long long blocks = (long long)a.tiles * a.kv_heads * a.sequences * a.splits;
+    kernel<<<(unsigned)blocks, S::kThreads, S::kBytes, stream>>>(a, mq, mk, mv, mo);
+    if (const int rc = ofe::launched()) return rc;
+    return join<T>(a, stream);
+}
+
+template <class T, int LK, int R>
+int launch_few(const Args &a, cudaStream_t stream) {
+    const long long blocks = (long long)a.kv_heads * a.sequences * a.splits;
+    attention_few_kernel<T, LK, R><<<(unsigned)blocks, FewShape<LK, R>::kThreads, 0, stream>>>(a);
+    if (const int rc = ofe::launched()) return rc;
+    return join<T>(a, stream);
+}
+template <class T>
+int run_few(const Args &a, cudaStream_t stream) {
+    if (a.head_dim > 64) return launch_few<T, 16, 1>(a, stream);
+    return a.group == 1 ? launch_few<T, 8, 1>(a, stream) : launch_few<T, 8, 2>(a, stream);
+}
+
 template <class T>
 int launch_for(const openfish_b200_attention_t *p, const Args &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const CUtensorMap &mo, int halves, cudaStream_t stream) {
-    if (p->head_dim <= 64) return launch<T, 64, 1>(a, mq, mk, mv, mo, stream);
-    return halves == 1 ? launch<T, 128, 1>(a, mq, mk, mv, mo, stream) : launch<T, 128, 2>(a, mq, mk, mv, mo, stream);
+    if (p->head_dim <= 64) return launch_tiles<T, 64, 1>(a, mq, mk, mv, mo, stream);
+    return halves == 1 ? launch_tiles<T, 128, 1>(a, mq, mk, mv, mo, stream) : launch_tiles<T, 128, 2>(a, mq, mk, mv, mo, stream);
 }
 
 size_t part_bytes(const openfish_b200_attention_t *a, int splits) {
@@ -704,6 +883,7 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
         a.part_lse = a.part + a.splits * a.part_step * a.head_dim;
     }
     const bool bf16 = p->dtype == OPENFISH_B200_BF16;
+    if (few_for(p)) return bf16 ? run_few<__nv_bfloat16>(a, (cudaStream_t)stream) : run_few<__half>(a, (cudaStream_t)stream);
     CUtensorMap mq, mk, mv, mo;
     const int d = p->head_dim, hk = p->kv_heads;
     bool made = p->k_rows == 0  // no keys at all: the kernel copies nothing, but a map has to be one of something

@@ -331,3 +331,47 @@ def test_drawn_shapes(native_lib):
         window = r.choice([(-1, -1), (-1, 0), (r.randint(0, 300), r.randint(0, 300)), (r.randint(0, 300), -1)])
         q, k, v = make(sum(q_len), Hq, dim, dtype, n), make(sum(k_len), Hkv, dim, dtype, n + 1), make(sum(k_len), Hkv, dim, dtype, n + 2)
         check(native_lib, q, k, v, q_len, k_len, window, r.choice([None, 0.3]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [8, 40, 64, 72, 128])
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5])
+def test_single_tokens(native_lib, dtype, dim, group):
+    # lengths around what a warp and a block take at a time, in a cache with room; what is not seen is no number
+    lens = [0, 1, 2, 3, 4, 5, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 1000, 7]
+    S, room = len(lens), 1003
+    q, k, v = make(S, 3 * group, dim, dtype, 1), make(S * room, 3, dim, dtype, 2), make(S * room, 3, dim, dtype, 3)
+    for s, n in enumerate(lens):
+        k[s * room + n : (s + 1) * room], v[s * room + n : (s + 1) * room] = math.nan, math.inf
+    for window in ((-1, 0), (0, 0), (64, -1), (100, 3)):
+        got = check(native_lib, q, k, v, [1] * S, [room] * S, window, k_used=lens)
+        assert (got[0] == 0).all()
+    # tokens that are not there
+    check(native_lib, q, k, v, [1] * S, [room] * S, k_used=lens, q_used=[n % 3 - 1 for n in range(S)], max_q=1)
+
+
+@pytest.mark.parametrize("heads,dim", [(2, 64), (1, 128)])
+@pytest.mark.parametrize("keys", [50, 5000])
+def test_single_tokens_with_large_scores_and_no_numbers(native_lib, heads, dim, keys):
+    q, k, v = make(1, heads, dim, torch.bfloat16, 1, 0.1), make(keys, 1, dim, torch.bfloat16, 2, 0.1), make(keys, 1, dim, torch.bfloat16, 3)
+    q[:, :, 0] = 8.0
+    for slope in (0.05, -0.05):
+        k[:, 0, 0] = (torch.arange(keys, device="cuda") * slope).to(k.dtype)
+        check(native_lib, q, k, v, [1], [keys], scale=1.0)
+    k[:, 0, 0] = 0
+    k[keys // 2, 0, 0] = 60.0
+    check(native_lib, q, k, v, [1], [keys], scale=1.0)
+    at = [starts([1])[1], starts([keys])[1], 1, keys]
+    for n in (0, keys // 3, keys - 1):
+        # a score of no number, and of infinity: no result; of minus infinity: no part
+        for bad in (math.nan, math.inf):
+            k2 = k.clone()
+            k2[n, 0, 0] = bad
+            assert torch.isnan(native_lib.attention(q, k2, v, *at)).all()
+        k2, v2 = k.clone(), v.clone()
+        k2[n, 0, 0], v2[n] = -math.inf, 0
+        keep = [j for j in range(keys) if j != n]
+        ref = attention_reference(q, k[keep], v[keep], [0, 1], [0, keys - 1])
+        assert close(native_lib.attention(q, k2, v2, *at), ref[0], attention_bound(ref, torch.bfloat16, keys))
+    k[:, 0, 0] = -math.inf
+    assert torch.isnan(native_lib.attention(q, k, v, *at)).all()
