@@ -56,6 +56,7 @@ def _packer(args):
 
 
 _pack_attention, _pack_matmul_i8, _pack_norm = _packer(AttentionArgs), _packer(MatmulI8Args), _packer(NormArgs)
+_pack_room = struct.Struct("@PN").pack  # the last fields of AttentionArgs: the workspace
 
 
 def declare(L):
@@ -99,7 +100,7 @@ def _tensor(name, x, dims):
 def _want(name, x, shape, dtype, device):
     """The address of a CUDA tensor of this shape, type and device (its index) whose rows are contiguous."""
     if (isinstance(x, _torch.Tensor) and x.dtype is dtype and x.get_device() == device and x.shape == shape
-            and (not shape or shape[-1] < 2 or x.stride(-1) == 1)):
+            and (not shape or shape[-1] < 2 or x.stride()[-1] == 1)):
         return x.data_ptr()
     if not isinstance(x, _torch.Tensor) or not x.is_cuda or x.dtype is not dtype:
         raise TypeError("%s must be a CUDA %s tensor" % (name, dtype))
@@ -164,14 +165,17 @@ def attention(q, k, v, q_start, k_start, max_q, max_k, q_used=None, k_used=None,
         with around:
             return attention(q, k, v, q_start, k_start, max_q, max_k, q_used, k_used, causal, window, scale, out, workspace)
     if out is None:
-        out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     fields = _attention_fields(q, k, v, q_start, k_start, max_q, max_k, out, q_used, k_used, causal, window, scale)
+    args = _pack_attention(*fields, 0, 0)
     if workspace is None:
-        need = L.openfish_b200_attention_workspace(_pack_attention(*fields, 0, 0))
+        need = L.openfish_b200_attention_workspace(args)
         if need:  # the stream's allocator takes it back in order
-            workspace = _torch.empty(need, dtype=_torch.uint8, device=q.device)
-    room = (0, 0) if workspace is None else (_want("workspace", workspace, workspace.shape, _torch.uint8, device), workspace.numel())
-    L.openfish_b200_attention(_torch._C._cuda_getCurrentRawStream(device), _pack_attention(*fields, *room))
+            workspace = q.new_empty(need, dtype=_torch.uint8)
+    if workspace is not None:
+        room = _pack_room(_want("workspace", workspace, workspace.shape, _torch.uint8, device), workspace.numel())
+        args = args[: -len(room)] + room
+    L.openfish_b200_attention(_torch._C._cuda_getCurrentRawStream(device), args)
     _check(L)
     return out
 
@@ -201,7 +205,7 @@ def matmul_i8(x, x_scale, w, w_scale, bias=None, dtype=None, out=None, stream=No
     (rows, depth), cols = x.shape, w.shape[0]
     if out is None:
         dtype = dtype or _torch.float16
-        out = _torch.empty((rows, cols), dtype=dtype, device=x.device)
+        out = x.new_empty((rows, cols), dtype=dtype)
     elif dtype is None:
         dtype = out.dtype
     int8, float32 = _torch.int8, _torch.float32
@@ -230,14 +234,14 @@ def norm(x, kind, weight=None, bias=None, eps=1e-5, residual=None, residual_scal
     dtype, shape = x.dtype, x.shape
     rows, width = shape
     if out is None:
-        out = _torch.empty(shape, dtype=dtype, device=x.device)
+        out = x.new_empty(shape)
     q = q_scale = None
     if quantize:
         stride = (width + 15) // 16 * 16
-        q = _torch.empty((rows, stride), dtype=_torch.int8, device=x.device)
+        q = x.new_empty((rows, stride), dtype=_torch.int8)
         if stride != width:
             q = q[:, :width]
-        q_scale = _torch.empty(rows, dtype=_torch.float32, device=x.device)
+        q_scale = x.new_empty(rows, dtype=_torch.float32)
     L.openfish_b200_norm(_torch._C._cuda_getCurrentRawStream(device), _pack_norm(
         _code(dtype), NORM_KINDS[kind], width, eps, residual_scale, rows, _want("x", x, shape, dtype, device),
         0 if residual is None else _want("residual", residual, shape, dtype, device),
