@@ -288,17 +288,22 @@ void launch(const NormArgs<T> &a, int threads, int sms, cudaStream_t stream) {
     norm_kernel<T, V, CH, BLOCK, SHIFT><<<(unsigned)blocks, threads, 0, stream>>>(a);
 }
 
-// A warp to a row while 4 packs (of one element: 16) to a lane hold it, else a block with as few packs to a thread as 1024
-// threads allow.
+// A warp to a row while 4 packs (of one element: 16) to a lane hold it, else a block with a few packs to a thread, so that an SM has several
+// rows and as many packs on their way as its registers hold.  Layer norm with a residual, us: 30000 rows of 2048 with two packs to a thread 74,
+// with one 88, and by warps with eight 88; 12000 of 4096 68, 83; 8000 of 8192 95, 130 (where rows start anywhere there is more to do for
+// a pack, and one is better: 8000 of 5001 84, with two 90).  Beyond 8192, where one would take more than 1024 threads, four: 4000 of
+// 9000 59, with four to each of 1024 threads 121; 2000 of 16000 56, 76.
 template <class T, int V, bool SHIFT>
 void dispatch(const NormArgs<T> &a, int sms, cudaStream_t stream) {
     const int packs = (a.width + V - 1) / V + SHIFT;
     constexpr int S = V == 8 ? 1 : 4;  // single elements are an eighth of a pack: more of them
+    constexpr int B = V == 8 && !SHIFT ? 2 : S;
     if (packs <= 32 * S) launch<T, V, S, false, SHIFT>(a, 128, sms, stream);
     else if (packs <= 64 * S) launch<T, V, 2 * S, false, SHIFT>(a, 128, sms, stream);
     else if (packs <= 96 * S) launch<T, V, 3 * S, false, SHIFT>(a, 128, sms, stream);
     else if (packs <= 128 * S) launch<T, V, 4 * S, false, SHIFT>(a, 128, sms, stream);
-    else if (packs <= 1024 * S) launch<T, V, S, true, SHIFT>(a, ((packs + S - 1) / S + 31) / 32 * 32, sms, stream);
+    else if (packs <= 1024 * S) launch<T, V, B, true, SHIFT>(a, ((packs + B - 1) / B + 31) / 32 * 32, sms, stream);
+    else if (V == 8 && packs <= 4096) launch<T, V, 4, true, SHIFT>(a, ((packs + 3) / 4 + 31) / 32 * 32, sms, stream);
     else launch<T, V, 4 * (8 / V) + SHIFT, true, SHIFT>(a, 1024, sms, stream);
 }
 

@@ -158,3 +158,15 @@ def test_captured_and_on_another_stream(native_lib):
     x.copy_(make(64, 512, torch.float16, 3))
     graph.replay()
     assert torch.equal(out, native_lib.norm(x, "layer", residual=r))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1032, 1040, 1536, 2504, 4088, 8184, 8192, 8200, 9000, 9001, 12289, 16384, 16392, 20001, 24576])
+def test_wide_rows_in_turn(native_lib, dtype, width):
+    # more rows than blocks are launched for, and a few; in place
+    for rows in (5, 1500):
+        x, r = make(rows, width, dtype, 1), make(rows, width, dtype, 2)
+        w, b = make(1, width, dtype, 3, 0.2, 1.0)[0], make(1, width, dtype, 4, 0.1)[0]
+        got, q, scale = check(native_lib, x, "layer", w, b, residual=r, residual_scale=2.4)
+        again = native_lib.norm(x, "layer", w, b, residual=r, residual_scale=2.4, out=x, quantize=True)
+        assert torch.equal(again[0], got) and torch.equal(again[1], q) and torch.equal(again[2], scale)
