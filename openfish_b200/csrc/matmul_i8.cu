@@ -62,7 +62,7 @@ struct Walk {  // the tiles in the order in which they are taken: stripes of 8 t
     }
 };
 
-template <class T, int CG, int BN>
+template <class T, int CG, int BN, int KS>
 __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel(const Args a, const Walk walk, const __grid_constant__ CUtensorMap map_x,
                                                                                  const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out) {
     using S = Shape<CG, BN>;
@@ -77,10 +77,36 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 2 ? blockIdx.x & 1 : 0;
-    const int group = blockIdx.x / CG, groups = gridDim.x / CG;
+    const int slice = KS > 1 ? blockIdx.x % KS : 0;
+    const int group = blockIdx.x / (CG * KS), groups = gridDim.x / (CG * KS);
     const int tiles = walk.tiles_m * walk.tiles_n;
-    const int steps = (a.depth + 127) / 128;
+    const int all_steps = (a.depth + 127) / 128, from = all_steps * slice / KS, steps = all_steps * (slice + 1) / KS;  // of the depth
 
+    // With KS slices of the depth, each block of the cluster has every KSth row of the results: these rows, this column and the
+    // seven behind it to a thread.
+    constexpr int kMine = KS > 1 ? 128 / KS * 8 / S::kThreads + (KS > 4) : 1;
+    float my_xs[kMine];
+    float2 my_ws[4], my_bias[4];
+    int my_row = 0, my_n = 0, tile_m = 0;
+    if (KS > 1) {
+        int tm, tn;
+        walk.at(group, &tm, &tn);
+        tile_m = tm * 128;
+        my_row = threadIdx.x / 8 * KS + slice;
+        my_n = tn * BN + threadIdx.x % 8 * 8;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int row = tile_m + my_row + i * S::kThreads / 8 * KS;
+            my_xs[i] = row < a.rows ? a.x_scale[row] : 0.f;
+        }
+        const T *const bias = static_cast<const T *>(a.bias);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float ws = my_n + e < a.cols ? a.w_scale[my_n + e] : 0.f, b = bias && my_n + e < a.cols ? ofe::to_float(bias[my_n + e]) : 0.f;
+            if (e & 1) my_ws[e / 2].y = ws, my_bias[e / 2].y = b;
+            else my_ws[e / 2].x = ws, my_bias[e / 2].x = b;
+        }
+    }
     if (threadIdx.x == 0) {
         *given_up = 0;
         for (int i = 0; i < S::kStages; ++i) {
@@ -112,7 +138,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
             int tm, tn;
             walk.at(t, &tm, &tn);
             const int m = tm * 128 * CG + rank * 128, n = tn * BN + rank * S::kRowsB;
-            for (int k = 0; k < steps; ++k, ++issued) {
+            for (int k = from; k < steps; ++k, ++issued) {
                 fine = tc5::wait_warp(&empty[stage], turn ^ 1, given_up, &g_status);
                 if (!fine) break;
                 uint8_t *const to = base + stage * S::kStageBytes;
@@ -143,13 +169,13 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
         for (int t = group; t < tiles && fine; t += groups, ++j) {
             const uint32_t sum = tmem + (j & 1) * BN;
             fine = tc5::wait_warp(&sum_empty[j & 1], ((j >> 1) & 1) ^ 1, given_up, &g_status);
-            for (int k = 0; k < steps && fine; ++k) {
+            for (int k = from; k < steps && fine; ++k) {
                 fine = tc5::wait_warp(&full[stage], turn, given_up, &g_status);
                 tc5::after_sync();
                 const uint64_t da = base_a + (uint32_t)(stage * (S::kStageBytes >> 4)), db = base_b + (uint32_t)(stage * (S::kStageBytes >> 4));
                 if (fine && tc5::elect()) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) tc5::mma_i8<CG>(sum, da + 2 * q, db + 2 * q, idesc, k > 0 || q > 0);
+                    for (int q = 0; q < 4; ++q) tc5::mma_i8<CG>(sum, da + 2 * q, db + 2 * q, idesc, k > from || q > 0);
                     if (CG == 1) tc5::commit(&empty[stage]);
                     else tc5::commit_pair(&empty[stage]);
                     if (k + 1 == steps) {
@@ -187,19 +213,21 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                 next[i].y = bias && n < a.cols ? ofe::to_float(bias[n]) : 0.f;
             }
         };
-        fetch(group);
+        if (KS == 1) fetch(group);
         int j = 0;
         for (int t = group; t < tiles; t += groups, ++j) {
             const int m0 = next_m0, n0 = next_n0;
             const float xs = next_xs;
-            __syncwarp();  // the last tile's scales have been read
+            if (KS == 1) {
+                __syncwarp();  // the last tile's scales have been read
 #pragma unroll
-            for (int i = 0; i < S::kPart / 32; ++i) {
-                scales[i * 32 + lane] = next[i].x;
-                biases[i * 32 + lane] = next[i].y;
+                for (int i = 0; i < S::kPart / 32; ++i) {
+                    scales[i * 32 + lane] = next[i].x;
+                    biases[i * 32 + lane] = next[i].y;
+                }
+                __syncwarp();
+                if (t + groups < tiles) fetch(t + groups);
             }
-            __syncwarp();
-            if (t + groups < tiles) fetch(t + groups);
             if (!tc5::wait_warp(&sum_full[j & 1], (j >> 1) & 1, given_up, &g_status)) break;
             tc5::after_sync();
 #pragma unroll 1
@@ -207,6 +235,14 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                 const uint32_t sum = tmem + ((uint32_t)(quarter * 32) << 16) + (j & 1) * BN + part * S::kPart + c;
                 uint32_t v[2][32];
                 tc5::ld64(v[0], v[1], sum);
+                if (KS > 1) {
+                    // a slice's sums, where its tiles were (all of them have been read)
+#pragma unroll
+                    for (int p = 0; p < 16; ++p)
+                        *reinterpret_cast<uint4 *>(base + (quarter * 32 + lane) * 256 + ((p ^ (lane & 7)) << 4)) =
+                            make_uint4(v[p >> 3][(p & 7) * 4], v[p >> 3][(p & 7) * 4 + 1], v[p >> 3][(p & 7) * 4 + 2], v[p >> 3][(p & 7) * 4 + 3]);
+                    continue;
+                }
                 if (c + 64 >= S::kPart) {  // the accumulator has been read: the next tile's sums may go there
                     tc5::before_sync();
                     __syncwarp();
@@ -285,12 +321,45 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
     __syncwarp();
     tc5::before_sync();
     __syncthreads();
-    if (CG == 2) tc5::cluster_sync();
+    if (CG == 2 || KS > 1) tc5::cluster_sync();
     tc5::after_sync();
+    if (KS > 1) {
+        const uint32_t at = tc5::smem_u32(base);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int row = my_row + i * S::kThreads / 8 * KS;
+            if (row >= 128 || tile_m + row >= a.rows) continue;
+            const int c = threadIdx.x % 8 * 2;
+            int4 lo = make_int4(0, 0, 0, 0), hi = lo;
+#pragma unroll
+            for (int z = 0; z < KS; ++z) {
+                const int4 p = tc5::load_peer(at + row * 256 + ((c ^ (row & 7)) << 4), z), q = tc5::load_peer(at + row * 256 + (((c + 1) ^ (row & 7)) << 4), z);
+                lo.x += p.x, lo.y += p.y, lo.z += p.z, lo.w += p.w;
+                hi.x += q.x, hi.y += q.y, hi.z += q.z, hi.w += q.w;
+            }
+            const float2 sum[4] = {{(float)lo.x, (float)lo.y}, {(float)lo.z, (float)lo.w}, {(float)hi.x, (float)hi.y}, {(float)hi.z, (float)hi.w}};
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = ofe::fma2(ofe::mul2(sum[e], {my_xs[i], my_xs[i]}), my_ws[e], my_bias[e]);
+                o[e] = ofe::pack<T>(f.x, f.y);
+            }
+            uint16_t *const out = static_cast<uint16_t *>(a.out) + (long long)(tile_m + row) * a.out_stride + my_n;
+            if (a.by_copy && my_n + 8 <= a.cols) {
+                *reinterpret_cast<uint4 *>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (my_n + e < a.cols) out[e] = (uint16_t)(o[e / 2] >> (e & 1) * 16);
+            }
+        }
+        __syncwarp();
+        tc5::cluster_sync();  // a block's memory stays until the others have read it
+    }
     if (warp == 1) tc5::tmem_free<CG>(tmem, S::kColumns);
 }
 
-template <class T, int CG, int BN>
+template <class T, int CG, int BN, int KS = 1>
 int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
     using S = Shape<CG, BN>;
     CUtensorMap mx, mw, mo;
@@ -301,7 +370,7 @@ int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
         return tc5::make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
     };
     bool made = map8(&mx, a.x, a.rows, a.depth, a.x_stride, 128) && map8(&mw, a.w, a.cols, a.depth, a.w_stride, S::kRowsB);
-    if (made && a.by_copy) {
+    if (made && a.by_copy && KS == 1) {
         const cuuint64_t dims[2] = {(cuuint64_t)a.cols, (cuuint64_t)a.rows};
         const cuuint64_t strides[1] = {(cuuint64_t)(a.rows > 1 ? a.out_stride : (a.cols + 7) / 8 * 8) * 2};
         const cuuint32_t box[2] = {64, 32};
@@ -310,22 +379,22 @@ int launch_tiles(const Args &a, int sms, cudaStream_t stream) {
         mo = mw;
     }
     if (!made) return ofb_fail(OPENFISH_B200_ERR_CUDA, "the driver made no tensor map");
-    const auto kernel = matmul_tile_kernel<T, CG, BN>;
+    const auto kernel = matmul_tile_kernel<T, CG, BN, KS>;
     if (const int rc = ofe::cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes))) return rc;
     const Walk walk((a.rows + 128 * CG - 1) / (128 * CG), (a.cols + BN - 1) / BN);
     const long long tiles = (long long)walk.tiles_m * walk.tiles_n;
-    const int most = sms / CG;
+    const int most = sms / CG;  // (with slices there is a cluster to every tile)
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * CG));
+    cfg.gridDim = dim3((unsigned)((KS > 1 ? tiles * KS : (tiles < most ? tiles : most) * CG)));
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.x = CG * KS;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = CG > 1 ? 1 : 0;
+    cfg.numAttrs = CG * KS > 1 ? 1 : 0;
     return ofe::cuda_status(cudaLaunchKernelEx(&cfg, kernel, a, walk, mx, mw, mo));
 }
 
@@ -386,6 +455,10 @@ int launch_few(const Args &a, cudaStream_t stream) {
 // Of the tiles, those whose rounds over the SMs are estimated to end first: a start, and a time for every 128 of the depth of a
 // round.  Measured (us by 64, 128, 256 wide tiles, the chosen one first): 512 x 1536 x 512 4.3, 4.8, 6.6; 512 x 8192 x 1024 8.0 (256), 8.5, 11.8; 1003 x 2504 x
 // 1237 8.8 (256), 10.3, 11.0; 2048 x 1536 x 512 6.2 (128), 6.7, 6.8; 4096 x 4096 x 4096 45 (256), 62, 109.
+// Where there are few tiles and much depth, a cluster of 2, 4 or 8 blocks takes a tile, a slice of the depth to each (sums of integers: exact
+// in any order).  us by one, two, four, eight: 64 x 4096 x 4096 10.4, 8.2 (four do not fit); 64 x 1024 x 4096 10.5, 8.1, 6.6, 10.9 (eight blocks to 16 tiles do not
+// all find a place, so half the SMs bound these); 64 x 512 x 2048 6.9, 6.2, 5.6, 5.4; 64 x 256 x 16384 32.3, 18.9, 11.9, 8.6; 64 x 512 x 512
+// 4.1, 4.8, 4.9.
 template <class T>
 int run(const Args &a, int sms, cudaStream_t stream) {
     if (a.rows <= 1) return launch_few<T, 1>(a, stream);
@@ -397,6 +470,22 @@ int run(const Args &a, int sms, cudaStream_t stream) {
         return start + ceil(tiles / at_once) * ((a.depth + 127) / 128) * step;
     };
     const double t64 = estimate(128, 64, sms, 3.0, 0.25), t128 = estimate(128, 128, sms, 3.6, 0.30), t256 = estimate(256, 256, sms / 2, 5.4, 0.36);
+    const long long tiles = (long long)((a.rows + 127) / 128) * ((a.cols + 63) / 64);
+    int slices = 1;
+    double best = t64 < t128 ? t64 : t128;
+    if (t256 < best) best = t256;
+    const double joins[3] = {1.2, 1.6, 1.9};
+    for (int i = 0; i < 3; ++i) {
+        const int n = 2 << i, steps = (a.depth + 127) / 128;
+        const double time = 3.0 + joins[i] + (steps + n - 1) / n * 0.25;
+        if (tiles * n <= (n == 8 ? sms / 2 : sms) && steps >= n && time < best) {
+            best = time;
+            slices = n;
+        }
+    }
+    if (slices == 2) return launch_tiles<T, 1, 64, 2>(a, sms, stream);
+    if (slices == 4) return launch_tiles<T, 1, 64, 4>(a, sms, stream);
+    if (slices == 8) return launch_tiles<T, 1, 64, 8>(a, sms, stream);
     if (t64 <= t128 && t64 <= t256) return launch_tiles<T, 1, 64>(a, sms, stream);
     return t128 < t256 ? launch_tiles<T, 1, 128>(a, sms, stream) : launch_tiles<T, 2, 256>(a, sms, stream);
 }

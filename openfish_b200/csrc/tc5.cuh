@@ -53,6 +53,14 @@ __device__ __forceinline__ uint32_t of_first_block(uint32_t addr) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// 16 bytes of the same place in another block of the cluster.
+__device__ __forceinline__ int4 load_peer(uint32_t addr, uint32_t block) {
+    int4 v;
+    asm volatile(
+        "{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %4, %5;\n\tld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [at];\n\t}"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "r"(block) : "memory");
+    return v;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }

@@ -121,3 +121,41 @@ def test_from_tokens_to_product(native_lib):
     dx, dw = 0.5 * xs.double()[:, None], 0.5 * ws.double()[:, None]
     off = dx * w.double().abs().sum(1)[None, :] + x.double().abs().sum(1)[:, None] * dw.t() + 600 * dx * dw.t()
     assert ((got - want).abs() <= off * 1.001 + 2.0 ** -11 * got.abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(64, 4096, 4096), (9, 4096, 4097), (128, 4090, 8000), (100, 1024, 4096), (129, 1003, 3999), (16, 64, 131071), (64, 256, 16384), (37, 321, 16000),
+                                   (128, 512, 2048), (300, 70, 5000), (64, 1100, 130000), (12, 1, 9999)])
+def test_few_tiles_and_much_depth(native_lib, dtype, M, N, K):
+    for pad, bias in ((0, False), (16, True)):
+        x, w = rows8(M, K, 1, pad), rows8(N, K, 2, pad)
+        got = check(native_lib, x, w, dtype, torch.randn(N, device="cuda").to(dtype) if bias else None)
+        # results that go off the 16-byte boundaries, and nothing beside them
+        wide = torch.full((M, N + 5), 7.0, dtype=dtype, device="cuda")
+        if not bias:
+            assert torch.equal(check(native_lib, x, w, dtype, out=wide[:, 3 : N + 3]), got)
+            assert (wide[:, :3] == 7).all() and (wide[:, N + 3 :] == 7).all()
+    # sums at the ends of 32 bits
+    x.fill_(-128)
+    w.fill_(-128)
+    check(native_lib, x, w, dtype, xs=torch.full((M,), 2.0 ** -20, device="cuda"), ws=torch.full((N,), 2.0 ** -10, device="cuda"))
+
+
+def test_few_tiles_captured_and_on_two_streams(native_lib):
+    x, w = rows8(64, 4096, 1), rows8(1024, 4096, 2)
+    x2, xs, ws = rows8(64, 4096, 5), scales(64, 3), scales(1024, 4)
+    want = [native_lib.matmul_i8(t, xs, w, ws) for t in (x, x2)]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[native_lib.matmul_i8(t, xs, w, ws, stream=s) for t, s in zip((x, x2), side)] for _ in range(30)]
+    for s in side:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(g, v) for pair in got for g, v in zip(pair, want))
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(want[0])
+    with torch.cuda.graph(graph):
+        native_lib.matmul_i8(x, xs, w, ws, out=out)
+    x.copy_(x2)
+    graph.replay()
+    assert torch.equal(out, want[1])
+    native_lib.encoder_wait()
