@@ -38,7 +38,8 @@ static int bad_heads(const char *func, const char *name, const void *p, long lon
 static int elements_meet(long long rows, int heads, int head_dim, long long stride_row, long long stride_head) {
     if (rows < 2) return heads > 1 && stride_head < head_dim;
     if (heads < 2) return stride_row < head_dim;
-    if (stride_head <= stride_row) return stride_head < head_dim || stride_row < (heads - 1) * stride_head + head_dim;
+    /* (the inner stride first; by division, for a product of these may pass 64 bits) */
+    if (stride_head <= stride_row) return stride_head < head_dim || (stride_row - head_dim) / stride_head < heads - 1;
     return stride_row < head_dim || (stride_head - head_dim) / stride_row < rows - 1;
 }
 

@@ -147,3 +147,10 @@ def test_numbers_that_no_field_holds_are_refused(native_lib, pack, args, number)
     fields[1] = number
     with pytest.raises(ValueError):
         getattr(native_lib.encoder, pack)(*fields)
+
+
+def test_results_that_share_places_beyond_64_bits(native_lib, lib):
+    # 10^9 heads, 2^38 elements apart, in rows no further apart
+    a = attention(native_lib, q_heads=10 ** 9, kv_heads=1, sequences=1, max_q=1, q_stride_head=64, out_stride_row=1 << 38, out_stride_head=1 << 38)
+    lib.openfish_b200_attention(None, C.byref(a))
+    assert lib.openfish_b200_last_status() == LAYOUT and b"overlap" in lib.openfish_b200_error_text()
