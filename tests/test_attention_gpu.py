@@ -375,3 +375,54 @@ def test_single_tokens_with_large_scores_and_no_numbers(native_lib, heads, dim, 
         assert close(native_lib.attention(q, k2, v2, *at), ref[0], attention_bound(ref, torch.bfloat16, keys))
     k[:, 0, 0] = -math.inf
     assert torch.isnan(native_lib.attention(q, k, v, *at)).all()
+
+
+@pytest.mark.parametrize("S,keys", [(1, 9000), (40, 700), (300, 130)])
+def test_single_tokens_captured_strided_and_on_two_streams(native_lib, S, keys):
+    # heads of a packed tensor of queries, keys and values; results into rows with room between them
+    args, outs = [], []
+    for seed in (1, 11):
+        new, cache = make(S, 12, 64, torch.float16, seed), make(S * keys, 12, 64, torch.float16, seed + 1)
+        args.append((new[:, :4], cache[:, 4:8], cache[:, 8:], starts([1] * S)[1], starts([keys] * S)[1], 1, keys))
+    want = [native_lib.attention(*a, causal=True) for a in args]
+    for a, w in zip(args, want):
+        wide = torch.full((S, 5, 72), 7.0, dtype=torch.float16, device="cuda")
+        assert torch.equal(native_lib.attention(*a, causal=True, out=wide[:, :4, 8:]), w)
+        assert (wide[:, 4] == 7).all() and (wide[:, :, :8] == 7).all()
+        ref = attention_reference(*a[:3], list(range(S + 1)), [keys * s for s in range(S + 1)], window=(-1, 0))
+        assert close(w, ref[0], attention_bound(ref, torch.float16, keys))
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[native_lib.attention(*a, causal=True, stream=s) for a, s in zip(args, side)] for _ in range(20)]
+    for s in side:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(g, w) for pair in got for g, w in zip(pair, want))
+    # a step captured twice in a row: the second one's kernels follow the first one's join
+    graph, out, again = torch.cuda.CUDAGraph(), torch.empty_like(want[0]), torch.empty_like(want[0])
+    with torch.cuda.graph(graph):
+        native_lib.attention(*args[0], causal=True, out=out)
+        native_lib.attention(out, *args[0][1:], causal=True, out=again)
+    for a, b in zip(args[0][:3], args[1][:3]):
+        a.copy_(b)
+    second = native_lib.attention(want[1], *args[1][1:], causal=True)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want[1]) and torch.equal(again, second)
+
+
+def test_single_tokens_beyond_32_bits_of_elements(native_lib):
+    first = 2 ** 32 // 128
+    cache = torch.empty(2, first + 4000, 1, 128, dtype=torch.bfloat16, device="cuda")
+    for t, seed in zip(cache, (2, 3)):
+        t[:first].zero_()
+        t[first:] = make(4000, 1, 128, torch.bfloat16, seed)
+    q = make(2, 1, 128, torch.bfloat16, 1)
+    got = native_lib.attention(q, cache[0], cache[1], starts([1, 1])[1], starts([first, 4000])[1], 1, first)
+    ref = attention_reference(q[1:], cache[0][first:], cache[1][first:], [0, 1], [0, 4000])
+    assert close(got[1:], ref[0], attention_bound(ref, torch.bfloat16, 4000))
+    assert (got[0] == 0).all()
+    # one sequence all of that long, seen from its end
+    got = native_lib.attention(q[1:], cache[0], cache[1], starts([1])[1], starts([first + 4000])[1], 1, first + 4000, window=(3999, 0))
+    assert close(got, ref[0], attention_bound(ref, torch.bfloat16, 4000))
