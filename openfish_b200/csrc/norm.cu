@@ -84,6 +84,7 @@ __device__ __forceinline__ float reduce(float v, float *scratch, Op op) {
 template <class T, int V, int CH, bool BLOCK, bool SHIFT>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs<T> a) {
     __shared__ float scratch[32];
+    __shared__ uint64_t firsts[BLOCK && SHIFT ? CH : 1][32];  // the codes of each warp's first thread
     constexpr int P = (V + 1) / 2;
     const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31;
     const int lanes = BLOCK ? blockDim.x : 32;
@@ -243,30 +244,36 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 128) norm_kernel(const NormArgs
             if (V == 8) codes[c] = *reinterpret_cast<const uint64_t *>(o);
             else codes[c] = (uint8_t)o[0];
         }
+        if (BLOCK && SHIFT && a.q_packs) {
+            if ((lane & 31) == 0) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) firsts[BLOCK && SHIFT ? c : 0][lane >> 5] = codes[c];
+            }
+            __syncthreads();  // (what was there for the row before has been read: the largest |y| has been found since)
+        }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int at = place(c);
             if (V == 8 && !SHIFT) {
                 if (here(at)) *reinterpret_cast<uint64_t *>(q + at) = codes[c];
             } else if (V == 8 && a.q_packs) {
-                // the eight codes from the next boundary on: the end of these and the beginning of the next thread's (of the last
-                // thread in a warp: of the first one's next pack; in a block that is another warp, and the codes go one by one)
+                // the eight codes from the next boundary on: the end of these and the beginning of the next thread's (behind the last
+                // thread in a warp: the next warp's first one, or the first one's next pack)
                 uint64_t after = __shfl_down_sync(0xffffffffu, codes[c], 1);
-                const int in_warp = lane & 31, to = at + shift;
-                if (!BLOCK && CH > 1) {
+                const int to = at + shift;
+                if (BLOCK) {
+                    const int warp = lane >> 5;
+                    if ((lane & 31) == 31) after = warp + 1 < lanes >> 5 ? firsts[SHIFT ? c : 0][warp + 1] : firsts[SHIFT && c + 1 < CH ? c + 1 : 0][0];
+                } else if (CH > 1) {
                     const uint64_t first_next = __shfl_sync(0xffffffffu, codes[c + 1 < CH ? c + 1 : c], 0);
-                    if (in_warp == 31) after = first_next;
+                    if (lane == 31) after = first_next;
                 }
                 const uint64_t both = shift == 0 ? codes[c] : codes[c] >> (8 * shift) | after << (64 - 8 * shift);
-                const int mine = BLOCK && in_warp == 31 ? 8 - shift : 8;
-                if (mine == 8 && to + 8 <= a.width) {
+                if (to + 8 <= a.width) {
                     *reinterpret_cast<uint64_t *>(q + to) = both;
                 } else {
-                    for (int i = 0; i < mine && to + i < a.width; ++i) q[to + i] = (int8_t)(both >> (8 * i));
+                    for (int i = 0; to + i < a.width; ++i) q[to + i] = (int8_t)(both >> (8 * i));
                 }
-                if (BLOCK && in_warp == 0)
-                    for (int i = 0; i < shift; ++i)
-                        if (at + i >= 0 && at + i < a.width) q[at + i] = (int8_t)(codes[c] >> (8 * i));
             } else if (here(at)) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
