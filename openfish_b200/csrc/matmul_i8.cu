@@ -29,6 +29,7 @@ struct Args {
 // ---------------------------------------------------------------------------------------------------------------
 // Tiles of 128 * CG tokens by BN channels.  CG = 2: a pair of blocks on two neighbouring SMs shares one tile, each holding half of
 // the tokens and half of the channels' weights, so that a byte of shared memory is filled once and read by both.
+// KS > 1: a cluster of KS blocks shares a tile, each with a slice of the depth; at the end each reads the others' sums of its rows.
 //
 // Warps: 0 issues the copies, 1 the matrix instructions, the ones from 4 on (a quarter of the accumulator's 128 lanes and half
 // of its columns each) scale and store.  The accumulator is there twice, so that one tile's sums are stored while the next one's are
