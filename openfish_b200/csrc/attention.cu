@@ -106,6 +106,13 @@ struct Shape {
     static constexpr int kHalfColumns = kBuffers * kKeys + DP, kColumns = H * kHalfColumns, kOut = kBuffers * kKeys;
 };
 
+// Results beyond this are worked out again with weights in fp32.  A result is a mean of values, but by the tiles its weights are rounded to
+// 16 bits one by one and their sum is not, so that among the type's largest numbers it may come out beyond them: an infinity.
+template <class T>
+constexpr float kLargest = 65504.f;
+template <>
+constexpr float kLargest<__nv_bfloat16> = 0x1.fep127f;
+
 // One row again, by a warp, straight from its definition and reading only the keys that the row sees.  A matrix
 // instruction multiplies the values of masked keys by weights of zero, which is no zero where such a value is an infinity or NaN.
 template <class T>
@@ -480,7 +487,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
 #pragma unroll
                     for (int b = 0; b < 8; ++b) {
                         f[b] = sees ? __uint_as_float(o[e + b]) * back : 0.f;
-                        bad |= !(fabsf(f[b]) < INFINITY);
+                        bad |= !(fabsf(f[b]) <= kLargest<T>);
                     }
                     const uint4 packed = make_uint4(pack<T>(f[0], f[1]), pack<T>(f[2], f[3]), pack<T>(f[4], f[5]), pack<T>(f[6], f[7]));
                     if (by_copy) {
