@@ -37,6 +37,16 @@ __device__ int g_status;  // of the kernels on this device: a wait that ran out
 constexpr int kRows = 128;  // of a half
 constexpr int kKeys = 64;   // of a tile
 constexpr float kLazy = 8.f;  // a maximum may be outgrown by 2^8 before what has been summed is scaled
+// Weights are held as 2^kRoom of their size.  The smallest number of fp16 is 2^-24 and its steps there are as large: without the room a key
+// that the largest outweighs by more is lost or doubled (131072 keys of 2^-24.9 beside one of 1 whose value is zero: 0.0062 for 0.0033).  With
+// it an underflow costs at most 2^-30 of a row's largest weight.  More room would leave less above, and a row whose first tile shows it few of its
+// keys outgrows its maximum soon (windows of 257 keys, us with none, 5, 6, 7: 89.3, 89.7, 90.1, 91.4).
+template <class T>
+constexpr float kRoom = 5.f;
+template <>
+constexpr float kRoom<__nv_bfloat16> = 0.f;  // (goes down to 2^-133)
+// What a tile's weights may add up to when they are worked out with the maximum there was before: none of them can be beyond the type.
+constexpr float kMostOfTile = 65504.f;
 
 struct Args {
     const int32_t *q_start, *k_start, *q_used, *k_used;
@@ -79,7 +89,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// Two weights 2^(c s - c m) as the matrix unit takes them, added to their row's sum before they are rounded.
+// Two weights 2^(c s - c m + room) as the matrix unit takes them: its operands have 16 bits.  They are added to their row's sum in fp32, before they are
+// rounded (a sum of the rounded ones would take two conversions more for every two keys, in the loop that bounds the kernel).
 template <class T>
 __device__ __forceinline__ uint32_t weights(float u, float w, float c, float shift, float2 &sum) {
     float2 z = {fmaf(u, c, shift), fmaf(w, c, shift)};
@@ -372,7 +383,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                 if (!careful) {
                     uint32_t s[2][32], p[2][16];
                     tc5::ld64(s[0], s[1], s_at);
-                    const float shift = -m * a.c;
+                    const float shift = fmaf(-m, a.c, kRoom<T>);
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                             p[n][e] = weights<T>(__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1]), a.c, shift, sum[e & 1]);
                     sum[0] = add2(sum[0], sum[1]);
                     const float tile_sum = sum[0].x + sum[0].y;
-                    careful = __any_sync(0xffffffffu, !(tile_sum <= 32768.f));  // (nor if it is no number)
+                    careful = __any_sync(0xffffffffu, !(tile_sum <= kMostOfTile));  // (nor if it is no number)
                     if (!careful) {
                         tc5::st16(s_at, p[0]);
                         tc5::st16(s_at + 16, p[1]);
@@ -433,7 +444,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                             tc5::st16(o_at + n, o);
                         }
                     }
-                    const float shift = m == -INFINITY ? 0.f : -m * a.c;
+                    const float shift = m == -INFINITY ? 0.f : fmaf(-m, a.c, kRoom<T>);
                     float2 sum = {0.f, 0.f};
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
@@ -519,7 +530,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                             *reinterpret_cast<const uint4 *>(staged + (n >> 6) * kRows * 128 + lane * 128 + (((n >> 3 & 7) ^ (lane & 7)) << 4));
                 }
             }
-            float lse = sees ? m * a.c + log2f(l) : -INFINITY;
+            float lse = sees ? m * a.c + (log2f(l) - kRoom<T>) : -INFINITY;
             __syncwarp();
             for (uint32_t again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
                 const int who = __ffs(again) - 1;

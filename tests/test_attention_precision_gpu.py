@@ -1,12 +1,57 @@
-"""Attention in fp16 where roundings to 16 bits show: results at the type's largest number."""
+"""Attention over long key sequences in fp16, with bounds well below the results: weights below the type's smallest numbers, results
+at its largest.
+
+The bounds, from the definition (u = 2^-11, half a step of fp16; P|v| = sum p|v| over the keys a query sees):
+  u |out|                        the result's own rounding
+  u P|v|                         by tiles: a weight is rounded to 16 bits on its way into the matrix product
+  2^-18 (1 + |z|) P|v|           a score's fp32 sum (up to 128 terms), the exponential's argument and value
+  keys 2^-25 P|v|                sums over keys in fp32: by tiles keys / 16 additions into the accumulator, truncated at worst (2^-23 each), and keys / 64
+                                 into the weights' sum; by lanes keys / 8 of 2^-24 into each of the two, and a scaling every fourth
+  keys 2^-30 max|v|              by tiles: underflow.  A row's largest weight is held as 2^5 or more, half the smallest subnormal is 2^-25"""
 import math
 
 import pytest
 import torch
 
-from encoder_util import starts
+from encoder_util import attention_reference, close, starts
 
 pytestmark = pytest.mark.gpu
+U = 2.0 ** -11
+
+
+def make(rows, heads, dim, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(rows, heads, dim, generator=g, device="cuda").half()
+
+
+def bound_of(ref, keys, lanes):
+    out, weight, zmax, vmax = ref
+    b = U * out.abs() + (2.0 ** -18 * (1 + zmax) + keys * 2.0 ** -25) * weight + 2.0 ** -25
+    return b if lanes else b + U * weight * (1 + 2 * U) + keys * 2.0 ** -30 * vmax
+
+
+def by_lanes(Hq, Hkv, dim, queries):
+    return queries == 1 and (Hq == Hkv or (Hq == 2 * Hkv and dim <= 64))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_below_the_smallest_numbers_of_the_type(native_lib, dim):
+    # One key outweighs each of the others by 2^24.9, but not all of them together by much.  So many queries that no block's keys
+    # are split (a piece without the first key would have a scale of its own).
+    queries, heads, keys = 10000, 8, 131072
+    q = torch.zeros(queries, heads, dim, dtype=torch.float16, device="cuda")
+    q[:, :, :2] = 1.0
+    k, v = torch.zeros(keys, 1, dim, dtype=torch.float16, device="cuda"), make(keys, 1, dim, 3).abs()
+    k[1:, 0, 0], k[1:, 0, 1] = -24.875, -0.025
+    v[0] = 0
+    at = starts([queries])[1], starts([keys])[1], queries, keys
+    assert native_lib.attention_workspace_bytes(q, k, v, *at, scale=math.log(2)) == 0
+    got = native_lib.attention(q, k, v, *at, scale=math.log(2))
+    ref = attention_reference(q[:1], k, v, [0, 1], [0, keys], scale=math.log(2))
+    bound = bound_of(ref, keys, False)
+    assert (bound < 0.25 * ref[0]).all()
+    assert (got == got[:1, :1]).all()  # the same query all along
+    assert close(got[:1], ref[0], bound), "%g for %g" % (got[0, 0, 0], ref[0][0, 0, 0])
 
 
 @pytest.mark.parametrize("dim", [64, 128])
