@@ -360,12 +360,12 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             __syncwarp();
             if (lane == 0) tc5::arrive(q_ready);
         }
-        // ---- the keys this row sees, and between them the first and the last row of the warp (rows that are not there
-        // are given the last row's)
+        // ---- the keys this row sees, none if it is not there, and between them the first and the last row of the warp that are
         int my_lo, my_hi;
         window(a, a.by_group.quotient(min(r, rows - 1)), nq, nk, &my_lo, &my_hi);
         const int first_lo = __shfl_sync(0xffffffffu, my_lo, 0), first_hi = __shfl_sync(0xffffffffu, my_hi, 0);
         const int last_lo = __shfl_sync(0xffffffffu, my_lo, 31), last_hi = __shfl_sync(0xffffffffu, my_hi, 31);
+        if (!there) my_lo = my_hi = 0;
         float m = -INFINITY, l = 0.f;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, o_at = tmem + lanes + S::kOut;
         bool fine = true;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
                             p[n][e] = weights<T>(__uint_as_float(s[n][e * 2]), __uint_as_float(s[n][e * 2 + 1]), a.c, shift, sum[e & 1]);
                     sum[0] = add2(sum[0], sum[1]);
                     const float tile_sum = sum[0].x + sum[0].y;
-                    careful = __any_sync(0xffffffffu, !(tile_sum <= kMostOfTile));  // (nor if it is no number)
+                    careful = __any_sync(0xffffffffu, my_hi != 0 && !(tile_sum <= kMostOfTile));  // (nor if it is no number)
                     if (!careful) {
                         tc5::st16(s_at, p[0]);
                         tc5::st16(s_at + 16, p[1]);

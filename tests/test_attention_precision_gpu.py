@@ -1,5 +1,5 @@
 """Attention over long key sequences in fp16, with bounds well below the results: weights below the type's smallest numbers, results
-at its largest.
+at its largest; and rows whose values must not show in other rows' roundings.
 
 The bounds, from the definition (u = 2^-11, half a step of fp16; P|v| = sum p|v| over the keys a query sees):
   u |out|                        the result's own rounding
@@ -68,3 +68,25 @@ def test_results_at_the_largest_number_of_the_type(native_lib, dim, queries, key
     v = torch.full_like(k, sign * 65504.0)
     got = native_lib.attention(q, k, v, starts([queries])[1], starts([keys])[1], queries, keys, window=window, scale=math.log(2))
     assert (got == sign * 65504.0).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rows_behind_the_queries_have_no_part(native_lib, dim, group, dtype):
+    # what lies behind a sequence's last query (room that is not used yet) changes not a bit of the results before it
+    room, used, keys = 160, [100, 33, 1, 130], 1000
+    S, H = len(used), 2
+    q, k, v = make(S * room, H * group, dim, 1).to(dtype), make(S * keys, H, dim, 2).to(dtype), make(S * keys, H, dim, 3).to(dtype)
+    lens = torch.tensor(used, dtype=torch.int32, device="cuda")
+    there = torch.cat([torch.arange(room, device="cuda") < n for n in used])
+    results = []
+    for behind in (0.0, math.nan, math.inf, 300.0, None):
+        x = q.clone()
+        if behind is not None:
+            x[~there] = behind
+        else:
+            x[~there] *= 40
+        results.append(native_lib.attention(x, k, v, starts([room] * S)[1], starts([keys] * S)[1], room, keys, q_used=lens)[there])
+    for r in results[1:]:
+        assert torch.equal(r, results[0])
