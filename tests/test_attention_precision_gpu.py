@@ -1,5 +1,5 @@
 """Attention over long key sequences in fp16, with bounds well below the results: weights below the type's smallest numbers, results
-at its largest; and rows whose values must not show in other rows' roundings.
+at its largest, a piece of the keys left out; and rows whose values must not show in other rows' roundings.
 
 The bounds, from the definition (u = 2^-11, half a step of fp16; P|v| = sum p|v| over the keys a query sees):
   u |out|                        the result's own rounding
@@ -32,6 +32,41 @@ def bound_of(ref, keys, lanes):
 
 def by_lanes(Hq, Hkv, dim, queries):
     return queries == 1 and (Hq == Hkv or (Hq == 2 * Hkv and dim <= 64))
+
+
+def by_lanes(Hq, Hkv, dim, queries):
+    return queries == 1 and (Hq == Hkv or (Hq == 2 * Hkv and dim <= 64))
+
+
+@pytest.mark.parametrize("Hq,Hkv,dim", [(8, 8, 64), (8, 4, 32), (3, 3, 80), (2, 2, 128), (4, 1, 64), (8, 2, 128), (6, 2, 80), (40, 8, 32)])
+@pytest.mark.parametrize("queries", [1, 3, 200])
+@pytest.mark.parametrize("keys", [1666, 4097, 9000, 30001])
+def test_many_keys_within_bounds_that_reject_a_missing_piece(native_lib, Hq, Hkv, dim, queries, keys):
+    q, k, v = make(queries, Hq, dim, 1), make(keys, Hkv, dim, 2), make(keys, Hkv, dim, 3)
+    ref = attention_reference(q, k, v, [0, queries], [0, keys])
+    bound = bound_of(ref, keys, by_lanes(Hq, Hkv, dim, queries))
+    # zeros would not do, nor a result without a 64th of the keys (a split, or a tile of the shorter ones)
+    assert not close(torch.zeros_like(q), ref[0], bound)
+    assert (bound < 0.25 * ref[0].abs().amax(dim=(0, 2), keepdim=True)).all()
+    kept = torch.ones(keys, dtype=torch.bool, device="cuda")
+    kept[keys // 2 : keys // 2 + keys // 64] = False
+    some = attention_reference(q, k[kept], v[kept], [0, queries], [0, int(kept.sum())])
+    assert not close(some[0].half(), ref[0], bound)
+    got = native_lib.attention(q, k, v, starts([queries])[1], starts([keys])[1], queries, keys)
+    assert close(got, ref[0], bound), "over the bound by %g" % ((got.double() - ref[0]).abs() - bound).max()
+
+
+@pytest.mark.parametrize("Hq", [2, 8])
+@pytest.mark.parametrize("keys", [1000, 30001])
+def test_the_mean_of_many_values(native_lib, Hq, keys):
+    # scores of zero: weights that every type holds, so nothing is rounded but sums and the result
+    q = torch.zeros(3, Hq, 64, dtype=torch.float16, device="cuda")
+    k, v = make(keys, 2, 64, 2), make(keys, 2, 64, 3)
+    out, weight, zmax, vmax = attention_reference(q, k, v, [0, 3], [0, keys])
+    bound = U * out.abs() + keys * 2.0 ** -25 * weight + 2.0 ** -25
+    assert not close(torch.zeros_like(q), out, bound)
+    got = native_lib.attention(q, k, v, starts([3])[1], starts([keys])[1], 3, keys)
+    assert close(got, out, bound)
 
 
 @pytest.mark.parametrize("dim", [64, 128])
