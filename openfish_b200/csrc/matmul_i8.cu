@@ -43,7 +43,7 @@ struct Shape {
     static constexpr int kStages = BN == 64 ? 7 : 5;
     static constexpr int kOutBytes = kParts * 4 * 4096;    // a warp's 32 rows of 64 results, twice
     static constexpr int kScaleBytes = kParts * 4 * kPart * 8; // a warp's channel scales and biases
-    static constexpr int kBytes = 1024 + kStages * kStageBytes + kOutBytes + kScaleBytes + (2 * kStages + 5) * 8 + 8;
+    static constexpr int kBytes = 1024 + kStages * kStageBytes + kOutBytes + kScaleBytes + (2 * kStages + 5) * 8 + 16;
     static constexpr int kColumns = 2 * BN;                    // of tensor memory, a power of two
 };
 
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
     uint64_t *const full = reinterpret_cast<uint64_t *>(out_stage + S::kOutBytes + S::kScaleBytes);
     uint64_t *const empty = full + S::kStages, *const sum_full = empty + S::kStages, *const sum_empty = sum_full + 2, *const done = sum_empty + 2;
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
-    volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1), *const steps_issued = given_up + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 2 ? blockIdx.x & 1 : 0;
@@ -159,8 +159,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                 if (++stage == S::kStages) stage = 0, turn ^= 1;
             }
         }
-        // after a wait that ran out: the copies under way land before the block ends
-        if (!fine && rank == 0 && lane == 0) ofd::mbar_drain_bounded(full, S::kStages, issued, ofd::kDefaultWaitLimitNs);
+        if (lane == 0) *steps_issued = issued;
     } else if (warp == 1 && rank == 0) {
         constexpr uint32_t idesc = tc5::idesc_i8(128 * CG, BN);
         const uint64_t base_a = tc5::desc_k_major(tc5::smem_u32(base)), base_b = tc5::desc_k_major(tc5::smem_u32(base) + 128 * 128);
@@ -187,11 +186,6 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
                 __syncwarp();
                 if (++stage == S::kStages) stage = 0, turn ^= 1;
             }
-        }
-        if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
-            if (CG == 1) tc5::commit(done);
-            else tc5::commit_pair(done);
-            ofd::mbar_land(done, 0, 0, ofd::kDefaultWaitLimitNs);
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, part = (warp - 4) >> 2;
@@ -320,10 +314,31 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) matmul_tile_kernel
         if (lane == 0) tc5::store_wait_read<0>();
     }
     __syncwarp();
+    if (CG == 2 && lane == 0 && *given_up) tc5::store_peer_word(given_up, rank ^ 1, 1);  // a pair gives up together
+    __syncwarp();
     tc5::before_sync();
     __syncthreads();
     if (CG == 2 || KS > 1) tc5::cluster_sync();
     tc5::after_sync();
+    if (*given_up) {
+        // A wait has run out, whichever it was: what is under way lands before the block (or its pair) ends and gives its memory back.
+        if (warp == 0 && rank == 0 && lane == 0) {
+            const uint64_t since = ofd::global_timer_ns();
+            land_copies(
+                *steps_issued, CG == 2 ? tc5::load_peer_word(steps_issued, 1) : *steps_issued, S::kStages,
+                [&](int stage) { ofd::mbar_arrive_expect_tx(&full[stage], S::kStageBytes); },
+                [&](int stage) { tc5::complete_tx(&full[stage], S::kStageBytes); },
+                [&](int stage, uint32_t parity) { ofd::mbar_land(&full[stage], parity, since, ofd::kDefaultWaitLimitNs); });
+        } else if (warp == 1 && rank == 0) {
+            if (tc5::elect()) {  // (the thread that has issued them)
+                tc5::commit<CG>(done);
+                ofd::mbar_land(done, 0, 0, ofd::kDefaultWaitLimitNs);
+            }
+        }
+        __syncwarp();
+        if (CG == 2) tc5::cluster_sync();
+        else __syncthreads();
+    }
     if (KS > 1) {
         const uint32_t at = tc5::smem_u32(base);
 #pragma unroll

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "give_up.h"
 #include "of_device.cuh"
 
 namespace tc5 {
@@ -16,7 +17,7 @@ using ofd::mbar_try_wait;
 using ofd::smem_u32;
 
 // ---- waits.  A block's flag goes up when one of its waits has run out; from then on every wait that does not find its phase complete at once
-// returns false, every role leaves its loop, and the kernel ends in order.
+// returns false, every role leaves its loop, and the block, behind its last barrier, sees land what any of them has left under way (give_up.h).
 static __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status) {
     uint64_t t0 = 0;
     for (uint32_t spin = 1;; ++spin) {
@@ -60,6 +61,21 @@ __device__ __forceinline__ int4 load_peer(uint32_t addr, uint32_t block) {
         "{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %4, %5;\n\tld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [at];\n\t}"
         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "r"(block) : "memory");
     return v;
+}
+// A word of the same place in another block of the cluster, read and written.
+__device__ __forceinline__ int load_peer_word(const volatile int *at, uint32_t block) {
+    int v;
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %1, %2;\n\tld.shared::cluster.s32 %0, [at];\n\t}"
+                 : "=r"(v) : "r"(smem_u32(const_cast<const int *>(at))), "r"(block) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_peer_word(volatile int *at, uint32_t block, int v) {
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, %1;\n\tst.shared::cluster.s32 [at], %2;\n\t}"
+                 ::"r"(smem_u32(const_cast<int *>(at))), "r"(block), "r"(v) : "memory");
+}
+// Bytes that a barrier counts as there although no copy brings them.
+__device__ __forceinline__ void complete_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
@@ -208,9 +224,11 @@ __device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b,
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
-// An arrival at `bar` once all matrix instructions of this thread so far are done.
+// An arrival at `bar` of this block once all matrix instructions of this thread so far (of a block, of a pair) are done.
+template <int CG = 1>
 __device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // The same at the barriers of that place in both blocks of a pair.
 __device__ __forceinline__ void commit_pair(uint64_t *bar) {
