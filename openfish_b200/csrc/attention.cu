@@ -112,7 +112,7 @@ struct Shape {
     static constexpr bool kCopyWarp = DP == 128;                // a warp of its own for the copies, where registers allow one
     static constexpr int kThreads = 32 * (5 * H + kCopyWarp);
     static constexpr int kHalfBarriers = 2 * kBuffers + 3;      // s_full and p_ready of each S, q_ready, the last two o_done
-    static constexpr int kBytes = H * kQueryBytes + kStages * kStageBytes + (2 * kStages + H * (kHalfBarriers + 1)) * 8 + 8;
+    static constexpr int kBytes = H * kQueryBytes + kStages * kStageBytes + (2 * kStages + H * (kHalfBarriers + 2)) * 8 + 8;
     // columns of tensor memory, a power of two: S and O of each half
     static constexpr int kHalfColumns = kBuffers * kKeys + DP, kColumns = H * kHalfColumns, kOut = kBuffers * kKeys;
 };
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     extern __shared__ __align__(1024) uint8_t q_tiles[];  // the swizzle counts from 1024-byte boundaries
     uint8_t *const ring = q_tiles + H * S::kQueryBytes;
     uint64_t *const full = reinterpret_cast<uint64_t *>(ring + S::kStages * S::kStageBytes), *const empty = full + S::kStages;
-    uint64_t *const my_turn = empty + S::kStages, *const of_half = my_turn + H;
+    uint64_t *const my_turn = empty + S::kStages, *const ended = my_turn + H, *const of_half = ended + H;
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(of_half + H * S::kHalfBarriers);
     volatile int *const given_up = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             ofd::mbar_init(&full[i], 1);
             ofd::mbar_init(&empty[i], H);
         }
-        for (int i = 0; i < H; ++i) ofd::mbar_init(&my_turn[i], 1);
+        for (int i = 0; i < 2 * H; ++i) ofd::mbar_init(&my_turn[i], 1);  // (and `ended`)
         for (int i = 0; i < H * S::kHalfBarriers; ++i) {
             // s_full and o_done are a commit's, p_ready takes an arrival of each warp, and so does q_ready without a copy
             const int of = i % S::kHalfBarriers;
@@ -334,10 +334,6 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
             }
             __syncwarp();
             if (++stage == S::kStages) stage = 0, turn ^= 1;
-        }
-        if (!fine && lane == 0) {  // after a wait that ran out: the instructions under way end before the block does
-            tc5::commit(o_done);
-            ofd::mbar_land(o_done, 0, 0, ofd::kDefaultWaitLimitNs);
         }
     } else {
         const int begin = H == 1 ? 0 : from[x], end = H == 1 ? count : to[x];
@@ -552,13 +548,21 @@ __global__ void __launch_bounds__(Shape<DP, H>::kThreads, Shape<DP, H>::kBlocks)
     tc5::before_sync();
     __syncthreads();
     tc5::after_sync();
-    if (*given_up && threadIdx.x == 0) {  // the copies under way land before the block ends
-        for (int n = 0; n < H; ++n)
-            if (a.q_by_copy && to[n] > from[n]) ofd::mbar_land(of_half + n * S::kHalfBarriers + 2 * S::kBuffers, 0, 0, ofd::kDefaultWaitLimitNs / 16);
-        for (int n = 0; n < S::kStages; ++n) {
-            const uint64_t since = ofd::mbar_land(&full[n], 0, 0, ofd::kDefaultWaitLimitNs / 16);
-            ofd::mbar_land(&full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
+    if (*given_up) {
+        // A wait has run out, whichever it was: what is under way lands before the block ends and gives its memory back.
+        if (threadIdx.x == 0) {
+            for (int n = 0; n < H; ++n)
+                if (a.q_by_copy && to[n] > from[n]) ofd::mbar_land(of_half + n * S::kHalfBarriers + 2 * S::kBuffers, 0, 0, ofd::kDefaultWaitLimitNs / 16);
+            for (int n = 0; n < S::kStages; ++n) {
+                const uint64_t since = ofd::mbar_land(&full[n], 0, 0, ofd::kDefaultWaitLimitNs / 16);
+                ofd::mbar_land(&full[n], 1, since, ofd::kDefaultWaitLimitNs / 16);
+            }
+        } else if (warp >= 4 * H && warp < 5 * H && tc5::elect()) {  // (the thread that has issued the products)
+            tc5::commit(&ended[x]);
+            ofd::mbar_land(&ended[x], 0, 0, ofd::kDefaultWaitLimitNs);
         }
+        __syncwarp();
+        __syncthreads();
     }
     if (warp == 4 * H) tc5::tmem_free<1>(tmem, S::kColumns);
 }
