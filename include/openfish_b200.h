@@ -284,10 +284,18 @@ typedef struct openfish_b200_norm {
 } openfish_b200_norm_t;
 void openfish_b200_norm(void *cuda_stream, const openfish_b200_norm_t *args);
 
-/* Waits for cuda_stream and reports whether a kernel of the three operators has given up waiting for a copy or a matrix
- * instruction on this device since the last such call (OPENFISH_B200_ERR_DEVICE_WAIT; results queued since are then
- * meaningless).  The operators themselves do not wait and cannot tell.  Not while a capture is under way. */
+/* Waits for cuda_stream and reports whether a kernel of the three operators has given up waiting (after two seconds) for a copy or a matrix
+ * instruction on this device, on any stream and whichever thread queued it, since the calling thread's last such call, or, at its first, since
+ * its first call of the operator (OPENFISH_B200_ERR_DEVICE_WAIT; results queued since may be meaningless).  Every thread gets its own report of
+ * it, once; a thread that calls no operator hears of what no thread has been told.  The operators themselves do not wait and cannot tell.  Not
+ * while a capture is under way. */
 void openfish_b200_encoder_wait(void *cuda_stream);
+
+/* Self-check of that path: queues on cuda_stream, for attention (1), matmul_i8 (2) or both (3), a one-block kernel whose only act is a wait
+ * as theirs, limit_us microseconds long, on a barrier that nothing will ever complete (no copy is issued).  The next
+ * openfish_b200_encoder_wait then has to report OPENFISH_B200_ERR_DEVICE_WAIT, and the one after it nothing.  Nothing faults, traps or hangs.
+ * Returns an openfish_b200_status value; does not touch openfish_b200_last_status(). */
+int openfish_b200_selfcheck_encoder_wait(void *cuda_stream, int kernels, unsigned limit_us);
 
 /* The four helpers the reference's test driver (src/main.c:207-252,337-351) calls next to the
  * public API; the reference declares them in an internal header (src/decode_cuda.h:35-55).

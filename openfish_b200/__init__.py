@@ -105,6 +105,8 @@ def lib():
         L.openfish_b200_decode_static.restype = i
         L.openfish_b200_decode_static.argtypes = [i, i, i, vp, i, C.POINTER(Opt), vp, vp, vp]
         _encoder.declare(L)
+        L.openfish_b200_selfcheck_encoder_wait.restype = i
+        L.openfish_b200_selfcheck_encoder_wait.argtypes = [vp, i, C.c_uint]
         L.get_openfish_log_level.restype = i
         L.set_openfish_log_level.argtypes = [i]
         # Python callers get exceptions instead of the reference's exit(1)
@@ -308,5 +310,5 @@ def last_rotary_ms():
     return float(lib().openfish_b200_last_rotary_ms())
 
 
-from .encoder import attention, attention_workspace_bytes, encoder_wait, matmul_i8, norm, quantize_i8  # noqa: E402,F401
+from .encoder import attention, attention_workspace_bytes, encoder_wait, matmul_i8, norm, quantize_i8, selfcheck_encoder_wait  # noqa: E402,F401
 from .sharding import shard_range  # noqa: E402,F401

@@ -32,7 +32,9 @@ using ofe::add2;
 using ofe::fma2;
 using ofe::pack;
 
-__device__ int g_status;  // of the kernels on this device: a wait that ran out
+__device__ int g_status;  // how many waits of the kernels have run out on this device
+Reports g_reports;
+thread_local int t_known[Reports::kDevices];
 
 constexpr int kRows = 128;  // of a half
 constexpr int kKeys = 64;   // of a tile
@@ -876,8 +878,9 @@ extern "C" size_t ofb_attention_workspace(const openfish_b200_attention_t *a) {
 }
 
 extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
-    int sms = 0;
-    if (const int rc = ofe::sm_count(&sms)) return rc;
+    int sms = 0, device = 0;
+    if (const int rc = ofe::sm_count(&sms, &device)) return rc;
+    g_reports.begin(device, t_known);
     Args a;
     a.q_start = p->q_start; a.k_start = p->k_start; a.q_used = p->q_used; a.k_used = p->k_used;
     a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out;
@@ -922,4 +925,5 @@ extern "C" int ofb_attention(void *stream, const openfish_b200_attention_t *p) {
     return bf16 ? launch_for<__nv_bfloat16>(p, a, mq, mk, mv, mo, halves, (cudaStream_t)stream) : launch_for<__half>(p, a, mq, mk, mv, mo, halves, (cudaStream_t)stream);
 }
 
-extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }
+extern "C" int ofb_attention_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, g_reports, t_known, gave_up); }
+extern "C" int ofb_attention_status(int **word) { return ofe::cuda_status(cudaGetSymbolAddress((void **)word, g_status)); }

@@ -1,4 +1,4 @@
-// encoder_device.cuh -- what the encoder's operators share: their two types, the status word of a device, launches.
+// encoder_device.cuh -- what the encoder's operators share: their two types, the reports of waits that have run out, launches.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "encoder.h"
+#include "reports.h"
 
 namespace ofe {
 
@@ -75,22 +76,21 @@ inline int cuda_status(cudaError_t e) {
     return e == cudaSuccess ? OPENFISH_B200_OK : ofb_fail(OPENFISH_B200_ERR_CUDA, cudaGetErrorString(e));
 }
 inline int launched() { return cuda_status(cudaGetLastError()); }
-inline int sm_count(int *out) {
+// The current device's, and which one that is.
+inline int sm_count(int *out, int *device = nullptr) {
     int dev = 0;
     if (const int rc = cuda_status(cudaGetDevice(&dev))) return rc;
+    if (device) *device = dev;
     return cuda_status(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
 }
-// Waits for the stream, then reads a file's status word and clears it.
-inline int settle(cudaStream_t stream, const int &symbol, int *gave_up) {
-    int seen = 0;
-    const int none = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(&seen, symbol, sizeof(seen), 0, cudaMemcpyDeviceToHost, stream);
+// Waits for the stream, then reads a file's count of waits that have run out: whether that is news to the calling thread.
+inline int settle(cudaStream_t stream, const int &symbol, Reports &reports, int *known, int *gave_up) {
+    int seen = 0, dev = 0;
+    *gave_up = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&seen, symbol, sizeof(seen), 0, cudaMemcpyDeviceToHost, stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-    if (e == cudaSuccess && seen) {
-        e = cudaMemcpyToSymbolAsync(symbol, &none, sizeof(none), 0, cudaMemcpyHostToDevice, stream);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-    }
-    *gave_up = seen != 0;
+    if (e == cudaSuccess) *gave_up = reports.take(dev, known, seen);
     return cuda_status(e);
 }
 

@@ -14,7 +14,9 @@
 
 namespace {
 
-__device__ int g_status;  // of the kernels on this device: a wait that ran out
+__device__ int g_status;  // how many waits of the kernels have run out on this device
+Reports g_reports;
+thread_local int t_known[Reports::kDevices];
 
 struct Args {
     const int8_t *x, *w;
@@ -509,8 +511,9 @@ int run(const Args &a, int sms, cudaStream_t stream) {
 }  // namespace
 
 extern "C" int ofb_matmul_i8(void *stream, const openfish_b200_matmul_i8_t *p) {
-    int sms = 0;
-    if (const int rc = ofe::sm_count(&sms)) return rc;
+    int sms = 0, device = 0;
+    if (const int rc = ofe::sm_count(&sms, &device)) return rc;
+    g_reports.begin(device, t_known);
     Args a;
     a.x = p->x; a.w = p->w; a.x_scale = p->x_scale; a.w_scale = p->w_scale; a.bias = p->bias; a.out = p->out;
     a.x_stride = p->x_stride; a.w_stride = p->w_stride; a.out_stride = p->out_stride;
@@ -519,4 +522,5 @@ extern "C" int ofb_matmul_i8(void *stream, const openfish_b200_matmul_i8_t *p) {
     return p->dtype == OPENFISH_B200_F16 ? run<__half>(a, sms, (cudaStream_t)stream) : run<__nv_bfloat16>(a, sms, (cudaStream_t)stream);
 }
 
-extern "C" int ofb_matmul_i8_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, gave_up); }
+extern "C" int ofb_matmul_i8_settle(void *stream, int *gave_up) { return ofe::settle((cudaStream_t)stream, g_status, g_reports, t_known, gave_up); }
+extern "C" int ofb_matmul_i8_status(int **word) { return ofe::cuda_status(cudaGetSymbolAddress((void **)word, g_status)); }

@@ -6,10 +6,12 @@
 #include <math.h>
 
 #include "backend.h"
+#include "encoder.h"
 #include "fast_lse.cuh"
 #include "of_device.cuh"
 #include "openfish_b200.h"
 #include "scan.cuh"
+#include "tc5.cuh"
 
 namespace {
 
@@ -58,7 +60,35 @@ __global__ void wait_that_runs_out_kernel(int *status, uint64_t wait_ns) {
     }
 }
 
+// The same by a whole warp, in the encoder's form.
+__global__ void encoder_wait_that_runs_out_kernel(int *status, uint64_t wait_ns) {
+    __shared__ uint64_t bar;
+    __shared__ int given_up;
+    if (threadIdx.x == 0) {
+        given_up = 0;
+        ofd::mbar_init(&bar, 1);
+        ofd::mbar_fence_init();
+    }
+    __syncwarp();
+    tc5::wait_warp(&bar, 0u, &given_up, status, wait_ns);
+}
+
 }  // namespace
+
+extern "C" int openfish_b200_selfcheck_encoder_wait(void *cuda_stream, int kernels, unsigned limit_us) {
+    int *words[2] = {};
+    if (kernels < 1 || kernels > 3) return OPENFISH_B200_ERR_ARGUMENT;
+    if (kernels & 1)
+        if (const int rc = ofb_attention_status(&words[0])) return rc;
+    if (kernels & 2)
+        if (const int rc = ofb_matmul_i8_status(&words[1])) return rc;
+    for (int *word : words) {
+        if (!word) continue;
+        encoder_wait_that_runs_out_kernel<<<1, 32, 0, (cudaStream_t)cuda_stream>>>(word, 1000ull * limit_us);
+        if (cudaGetLastError() != cudaSuccess) return OPENFISH_B200_ERR_CUDA;
+    }
+    return OPENFISH_B200_OK;
+}
 
 cudaError_t of_launch_wait_that_runs_out(int *status, uint64_t wait_ns, cudaStream_t stream) {
     wait_that_runs_out_kernel<<<1, 32, 0, stream>>>(status, wait_ns);

@@ -16,9 +16,9 @@ namespace tc5 {
 using ofd::mbar_try_wait;
 using ofd::smem_u32;
 
-// ---- waits.  A block's flag goes up when one of its waits has run out; from then on every wait that does not find its phase complete at once
+// ---- waits.  `status` counts on the device how often one has run out.  A block's flag goes up when one of its waits has; from then on every wait that does not find its phase complete at once
 // returns false, every role leaves its loop, and the block, behind its last barrier, sees land what any of them has left under way (give_up.h).
-static __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status) {
+static __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status, uint64_t limit_ns) {
     uint64_t t0 = 0;
     for (uint32_t spin = 1;; ++spin) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -26,20 +26,20 @@ static __device__ __forceinline__ bool wait_slow(uint64_t *bar, uint32_t parity,
         if ((spin & 63u) == 0) {
             const uint64_t now = ofd::global_timer_ns();
             if (t0 == 0) t0 = now;
-            else if (now - t0 > ofd::kDefaultWaitLimitNs) {
+            else if (now - t0 > limit_ns) {
                 *given_up = 1;
-                atomicExch(status, ofd::kStatusWaitTimeout);
+                atomicAdd(status, 1);
                 return false;
             }
         }
     }
 }
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status) {
-    return mbar_try_wait(bar, parity) || wait_slow(bar, parity, given_up, status);
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status, uint64_t limit_ns = ofd::kDefaultWaitLimitNs) {
+    return mbar_try_wait(bar, parity) || wait_slow(bar, parity, given_up, status, limit_ns);
 }
 // By a whole warp, which carries on together.
-__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status) {
-    return __all_sync(0xffffffffu, wait(bar, parity, given_up, status));
+__device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity, volatile int *given_up, int *status, uint64_t limit_ns = ofd::kDefaultWaitLimitNs) {
+    return __all_sync(0xffffffffu, wait(bar, parity, given_up, status, limit_ns));
 }
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");

@@ -263,9 +263,18 @@ def quantize_i8(x, stream=None):
 
 def encoder_wait(stream=None):
     """openfish_b200_encoder_wait: waits for the stream (default: the current one) and raises if a kernel of these operators has
-    given up waiting on its device."""
+    given up waiting on its device since the calling thread's last such call (or its first call of the operator)."""
     L = _ready()
     stream = stream or _torch.cuda.current_stream()
     with _elsewhere(stream.device.index, None) or contextlib.nullcontext():
         L.openfish_b200_encoder_wait(stream.cuda_stream)
     _check(L)
+
+
+def selfcheck_encoder_wait(kernels=3, limit_us=1000, stream=None):
+    """openfish_b200_selfcheck_encoder_wait on the stream (default: the current one), for attention (1), matmul_i8 (2) or both: the status
+    code.  The next encoder_wait has to raise, the one after it not."""
+    L = _ready()
+    stream = stream or _torch.cuda.current_stream()
+    with _elsewhere(stream.device.index, None) or contextlib.nullcontext():
+        return int(L.openfish_b200_selfcheck_encoder_wait(stream.cuda_stream, kernels, limit_us))
