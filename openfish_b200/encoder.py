@@ -2,7 +2,9 @@
 sequences, the product of 8-bit integers, and the residual norm that feeds it.
 
 Tensors are torch CUDA tensors of one device; the calls queue their kernels on ``stream`` (a torch.cuda.Stream of that
-device; its current stream by default) and return.  Arguments that cannot be served raise before anything is queued:
+device; its current stream by default) and return.  On another stream than the current one, it is the caller who lets ``stream`` wait for what makes
+the inputs, and the current stream for the results; the memory of both is kept until the streams are done with it, so that no tensor has to be
+held on to.  Arguments that cannot be served raise before anything is queued:
 TypeError and ValueError for what is no such tensor, OpenfishError for what the library refuses.  The operators serve: no
 gradient passes through them.
 """
@@ -111,13 +113,32 @@ def _want(name, x, shape, dtype, device):
     raise ValueError("%s: the elements of a row must lie next to each other" % name)
 
 
-def _elsewhere(device, stream):
-    """What a call needs around it where it does not go to the current device's current stream: None, or a context."""
-    if stream is not None:
-        if stream.device.index != device:
-            raise ValueError("the stream is on %s, the tensors on cuda:%d" % (stream.device, device))
-        return _torch.cuda.stream(stream)
+def _elsewhere(device):
+    """What a call needs around it where it does not go to the current device: None, or a context."""
     return None if device == _torch.cuda.current_device() else _torch.cuda.device(device)
+
+
+def _of_device(stream, device):
+    if stream.device.index != device:
+        raise ValueError("the stream is on %s, the tensors on cuda:%d" % (stream.device, device))
+    return stream
+
+
+def _on_stream(stream, call, *tensors):
+    """call() on that stream, in whose allocations it makes its results.  The inputs' memory is not given to others before the stream is done with
+    it, nor the results' before the caller's current stream is."""
+    device = stream.device
+    current = _torch.cuda.current_stream(device)
+    with _torch.cuda.stream(stream):
+        results = call()
+    if stream != current:
+        for t in tensors:
+            if isinstance(t, _torch.Tensor):
+                t.record_stream(stream)
+        for t in results if isinstance(results, tuple) else (results,):
+            if t is not None:
+                t.record_stream(current)
+    return results
 
 
 def _check(L):
@@ -160,7 +181,11 @@ def attention(q, k, v, q_start, k_start, max_q, max_k, q_used=None, k_used=None,
     L = _ready()
     _tensor("q", q, 3)
     device = q.get_device()
-    around = _elsewhere(device, stream)
+    if stream is not None:
+        return _on_stream(_of_device(stream, device), lambda: attention(q, k, v, q_start, k_start, max_q, max_k, q_used, k_used, causal, window, scale,
+                                                                        out, workspace),
+                          q, k, v, q_start, k_start, q_used, k_used, out, workspace)
+    around = _elsewhere(device)
     if around is not None:
         with around:
             return attention(q, k, v, q_start, k_start, max_q, max_k, q_used, k_used, causal, window, scale, out, workspace)
@@ -185,7 +210,7 @@ def attention_workspace_bytes(q, k, v, q_start, k_start, max_q, max_k, q_used=No
     """openfish_b200_attention_workspace of that call."""
     L = _ready()
     fields = _attention_fields(q, k, v, q_start, k_start, max_q, max_k, q if out is None else out, q_used, k_used, causal, window, scale)
-    with _elsewhere(q.get_device(), None) or contextlib.nullcontext():
+    with _elsewhere(q.get_device()) or contextlib.nullcontext():
         need = L.openfish_b200_attention_workspace(_pack_attention(*fields, 0, 0))
     _check(L)
     return need
@@ -198,7 +223,9 @@ def matmul_i8(x, x_scale, w, w_scale, bias=None, dtype=None, out=None, stream=No
     _tensor("x", x, 2)
     _tensor("w", w, 2)
     device = x.get_device()
-    around = _elsewhere(device, stream)
+    if stream is not None:
+        return _on_stream(_of_device(stream, device), lambda: matmul_i8(x, x_scale, w, w_scale, bias, dtype, out), x, x_scale, w, w_scale, bias, out)
+    around = _elsewhere(device)
     if around is not None:
         with around:
             return matmul_i8(x, x_scale, w, w_scale, bias, dtype, out)
@@ -227,7 +254,10 @@ def norm(x, kind, weight=None, bias=None, eps=1e-5, residual=None, residual_scal
         raise ValueError("kind must be one of %s" % ", ".join(NORM_KINDS))
     _tensor("x", x, 2)
     device = x.get_device()
-    around = _elsewhere(device, stream)
+    if stream is not None:
+        return _on_stream(_of_device(stream, device), lambda: norm(x, kind, weight, bias, eps, residual, residual_scale, out, quantize),
+                          x, weight, bias, residual, out)
+    around = _elsewhere(device)
     if around is not None:
         with around:
             return norm(x, kind, weight, bias, eps, residual, residual_scale, out, quantize)
@@ -266,7 +296,7 @@ def encoder_wait(stream=None):
     given up waiting on its device since the calling thread's last such call (or its first call of the operator)."""
     L = _ready()
     stream = stream or _torch.cuda.current_stream()
-    with _elsewhere(stream.device.index, None) or contextlib.nullcontext():
+    with _elsewhere(stream.device.index) or contextlib.nullcontext():
         L.openfish_b200_encoder_wait(stream.cuda_stream)
     _check(L)
 
@@ -276,5 +306,5 @@ def selfcheck_encoder_wait(kernels=3, limit_us=1000, stream=None):
     code.  The next encoder_wait has to raise, the one after it not."""
     L = _ready()
     stream = stream or _torch.cuda.current_stream()
-    with _elsewhere(stream.device.index, None) or contextlib.nullcontext():
+    with _elsewhere(stream.device.index) or contextlib.nullcontext():
         return int(L.openfish_b200_selfcheck_encoder_wait(stream.cuda_stream, kernels, limit_us))
