@@ -290,7 +290,12 @@ def decode_wait(gpubuf):
 
 def rotary_emb_gpu(x_gpu, sin_gpu, cos_gpu, batch_size, seqlen, nheads, head_dim, rotary_half,
                    stride_batch, stride_seq, stride_head):
-    """openfish_rotary_emb_gpu on torch CUDA tensors (x float16 in place, sin/cos float32)."""
+    """openfish_rotary_emb_gpu on torch CUDA tensors (x float16 in place, sin/cos float32).  It runs on the legacy default stream, which
+    does not wait for torch's other streams: what is queued on the current one, if that is another, is waited for first.  Returns when it is
+    done."""
+    import torch
+    if torch._C._cuda_getCurrentRawStream(x_gpu.get_device()):
+        torch.cuda.current_stream(x_gpu.device).synchronize()
     (_lib or lib()).openfish_rotary_emb_gpu(x_gpu.data_ptr(), sin_gpu.data_ptr(), cos_gpu.data_ptr(),
                                             batch_size, seqlen, nheads, head_dim, rotary_half, stride_batch,
                                             stride_seq, stride_head)

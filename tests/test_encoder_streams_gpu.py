@@ -1,5 +1,5 @@
 """The encoder's operators on streams that are not their tensors' own: memory that is given back while a call still
-waits to run."""
+waits to run, and the rotary embedding behind work on a side stream."""
 import pytest
 import torch
 
@@ -61,3 +61,24 @@ def test_results_may_be_given_back_while_they_are_read(native_lib, which):
     for a, b in zip(copies, want):
         assert torch.equal(a, b)
     del fresh
+
+
+def test_rotary_on_what_a_side_stream_makes(native_lib):
+    # the embedding runs on the legacy default stream, which torch's side streams do not wait for nor are waited for by
+    T, H, D = 500, 8, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    first, then = (torch.randn(T, 3 * H, D, generator=g, device="cuda").half() for _ in range(2))
+    angle = torch.rand(T, D // 2, generator=g, device="cuda")
+    sin, cos = torch.sin(angle), torch.cos(angle)
+    args = (1, T, 2 * H, D, D // 2, T * 3 * H * D, 3 * H * D, D)
+    want = then.clone()
+    native_lib.rotary_emb_gpu(want, sin, cos, *args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(LONG)
+        first.copy_(then)
+        native_lib.rotary_emb_gpu(first, sin, cos, *args)
+        got = first.clone()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
