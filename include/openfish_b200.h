@@ -222,7 +222,7 @@ typedef struct openfish_b200_attention {
     int head_dim, q_heads, kv_heads;
     int sequences, max_q, max_k;
     int window_left, window_right;
-    float scale; /* above zero */
+    float scale; /* above zero, and finite in fp32 times log2(e) too: up to 2.3e38 */
     long long q_rows, k_rows;
     const int32_t *q_start, *k_start;
     const int32_t *q_used, *k_used; /* or NULL */

@@ -56,7 +56,8 @@ static int bad_attention_sizes(const char *func, const openfish_b200_attention_t
     if (a->q_rows > INT_MAX - 65536 || a->k_rows > INT_MAX - 65536 || a->max_k > INT_MAX / 4 || (double)a->max_q * a->q_heads > 1e9 ||
         ((double)a->max_q * a->q_heads / a->kv_heads / 128 + 1) * a->kv_heads * a->sequences > 1e9)
         return refuse(func, OPENFISH_B200_ERR_TOO_LONG, "more rows than the kernels count (2^31 rows, 2^29 keys and 10^9 query heads of one sequence, 10^9 tiles of 128)");
-    if (!(a->scale > 0.f) || isinf(a->scale)) return refuse(func, OPENFISH_B200_ERR_ARGUMENT, "scale must be finite and above zero");
+    if (!(a->scale > 0.f) || isinf(a->scale * 1.4426950408889634f)) /* (the kernels count in powers of two) */
+        return refuse(func, OPENFISH_B200_ERR_ARGUMENT, "scale must be above zero and, times log2(e), finite");
     if (a->window_left < -1 || a->window_right < -1)
         return refuse(func, OPENFISH_B200_ERR_ARGUMENT, "a window is -1 (no bound) or a number of keys");
     return 0;
