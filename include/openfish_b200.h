@@ -195,7 +195,8 @@ int openfish_b200_decode_static(int T, int N, int C, const void *scores_TNC, int
  *     preparation.
  *   - Strides are in elements.  Arguments that cannot be served are refused before anything is queued
  *     (openfish_b200_last_status, the library's error mode).
- *   - Sums, statistics and scales are held in 32 bits; a result is rounded to its type once. */
+ *   - Sums, statistics and scales are held in 32 bits; a result is rounded to its type once.  One rounding lies on the way: the matrix
+ *     instructions take attention's softmax weights p in 16 bits (see there). */
 enum openfish_b200_dtype { OPENFISH_B200_F16 = 0, OPENFISH_B200_BF16 = 1 };
 
 /* Attention over packed sequences.
@@ -207,7 +208,10 @@ enum openfish_b200_dtype { OPENFISH_B200_F16 = 0, OPENFISH_B200_BF16 = 1 };
  * queries): the sequences' ends fall together.  A window of -1 has no bound; window_right = 0 is causal attention,
  * both -1 attention over the whole sequence, and one query against many keys is the step of a decoder with a
  * cache.  <q, k> is a sum in fp32 before it is scaled; one beyond fp32 is an infinity, with what follows from that (a query all of whose keys give
- * -inf has no softmax: NaN).  A query that sees no key gets zeros.  Keys that a query does not see have no part in its result, whatever
+ * -inf has no softmax: NaN), and the same goes for a scaled one.  Sums over keys are formed in fp32, of weights p that are rounded to `dtype` on their way into
+ * the matrix product with v (half a step, 2^-11 of a weight in fp16, 2^-8 in bf16; in fp16 weights are good to 2^-30 of the query's largest besides); what they are divided by is the
+ * sum before that rounding.  Single tokens (max_q 1) with q_heads equal to kv_heads, or twice that and head_dim up to 64, are worked out without it.
+ * A query that sees no key gets zeros.  Keys that a query does not see have no part in its result, whatever
  * their values (infinities and NaN included).
  *
  * q [q_rows][q_heads][head_dim], k and v [k_rows][kv_heads][head_dim], out like q, all of type `dtype`, the head_dim
@@ -266,7 +270,8 @@ void openfish_b200_matmul_i8(void *cuda_stream, const openfish_b200_matmul_i8_t 
  *
  * weight and bias [width] or NULL (1 and 0; kind NONE takes neither).  out (or NULL): y in the type of x.  q (or NULL): y in
  * 8 bits, q = round(y * 127 / top) to nearest, ties to even, and q_scale[row] = top / 127 with top = max |y| of the row (from the unrounded y); a row of zeros gets
- * zeros and scale 0, a row with an infinity or NaN zeros and scale NaN.  width up to 32768.  out may be x or
+ * zeros and scale 0, a row with an infinity or NaN zeros and scale NaN.  A sum of squares beyond fp32 (values from about 10^19 on) is an infinity, and the row
+ * over its root zeros.  width up to 32768.  out may be x or
  * residual themselves (same pointer, same stride).  Rows of x and residual, weight and bias may be read up to the 16-byte boundaries around them,
  * what lies there is not used. */
 enum openfish_b200_norm_kind { OPENFISH_B200_NORM_NONE = 0, OPENFISH_B200_NORM_LAYER = 1, OPENFISH_B200_NORM_RMS = 2 };

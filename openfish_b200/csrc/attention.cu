@@ -13,7 +13,8 @@
 //   1 warp              asynchronous copies of the keys' and values' tiles (heads of up to 64: the last warp above)
 //
 // Tensor memory and registers decide how many halves there are to an SM, and only other halves' work fills the waits between a
-// tile's steps.  Heads of up to 64: S and O take 128 columns, four blocks of a half.  Heads of up to 128: O alone takes
+// tile's steps.  Heads of up to 64: S and O take 128 columns, four blocks of a half, of 96 registers a thread (56 bytes
+// do not fit and go through memory).  Heads of up to 128: O alone takes
 // that, so two halves, each with two S in turn: the next tile's S is formed while this tile's weights are worked out.  The
 // two share a block and its tiles, for the copies' way into shared memory and the products' way out of it are what bounds
 // these heads: 48 cycles for each 128 x 64 x 16 of Q K^T (6 KB), 64 for 128 x 128 x 16 of P V.  Where there are rows for one half only (single
