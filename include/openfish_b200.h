@@ -210,7 +210,7 @@ enum openfish_b200_dtype { OPENFISH_B200_F16 = 0, OPENFISH_B200_BF16 = 1 };
  * cache.  <q, k> is a sum in fp32 before it is scaled; one beyond fp32 is an infinity, with what follows from that (a query all of whose keys give
  * -inf has no softmax: NaN), and the same goes for a scaled one.  Sums over keys are formed in fp32, of weights p that are rounded to `dtype` on their way into
  * the matrix product with v (half a step, 2^-11 of a weight in fp16, 2^-8 in bf16; in fp16 weights are good to 2^-30 of the query's largest besides); what they are divided by is the
- * sum before that rounding.  Single tokens (max_q 1) with q_heads equal to kv_heads, or twice that and head_dim up to 64, are worked out without it.
+ * sum before that rounding.  A sum over keys beyond fp32 (bf16 values of more than 3.4 10^38 over the number of keys) is an infinity, although the mean may not be.  Single tokens (max_q 1) with q_heads equal to kv_heads, or twice that and head_dim up to 64, are worked out without it.
  * A query that sees no key gets zeros.  Keys that a query does not see have no part in its result, whatever
  * their values (infinities and NaN included).
  *
